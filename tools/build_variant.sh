@@ -11,7 +11,7 @@ python -m diffgraph_amd.build >/dev/null
 mkdir -p scratch
 C=diffgraph_amd/csrc
 for s in ${VARIANT_SOURCES:-spmm graph}; do
-  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Wall -Wno-unused-function "$@" -c $C/$s.hip -o scratch/${s}_$tag.o
+  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Wall -Wno-unused-function -Xclang -target-feature -Xclang -packed-fp32-ops "$@" -c $C/$s.hip -o scratch/${s}_$tag.o
 done
 objs=""
 for s in graph spmm fused diffusion wgrad losshead eval sampling spgemm optim linear comm; do
