@@ -22,6 +22,7 @@ DG_BWD_NORM_FEED = 32
 DG_ROWS_PARTIAL_ONLY, DG_ROWS_FULL_ONLY = 64, 128
 DG_OUT_PLANES, DG_IN_PLANES = 0x200, 0x400
 DG_ACC_SHARED = 0x800
+DG_F32, DG_BF16, DG_F16 = 0, 1, 2
 
 
 class DiffGraphHipError(RuntimeError):
@@ -177,6 +178,11 @@ SIGNATURES = {
     "dg_adam_multi": (C.c_int, [C.POINTER(C.c_void_p)] * 4 + [C.POINTER(C.c_int64), C.c_int32, C.c_void_p] + [C.c_float] * 5
                       + [C.c_void_p]),
     "dg_clear": (C.c_int, [C.c_void_p, C.c_size_t, C.c_void_p]),
+    "dg_embedding_lookup": (C.c_int, [C.c_void_p, C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_int32, C.c_int64,
+                                      C.c_float, C.c_void_p, C.c_void_p]),
+    "dg_embedding_grad_workspace": (C.c_size_t, [C.c_int64, C.c_int64, C.c_int32]),
+    "dg_embedding_grad": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_int32, C.c_int32,
+                                    C.c_float, C.c_int64, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     "dg_rec_head_bwd": (C.c_int, [C.c_void_p] * 6 + [C.c_int32] * 3 + [C.c_double, C.c_double, C.c_int32] + [C.c_void_p] * 10),
 }
 
@@ -225,6 +231,13 @@ def device_guard(device=None):
     if device.type != "cuda":
         raise DiffGraphHipError(f"graphs live on a GPU, got device {device}")
     return torch.cuda.device(device)
+
+
+def on_device(device):
+    """Context in which `device` (a tensor's) is the current GPU, so that a launch on its stream goes there."""
+    import contextlib
+    import torch
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def stream_ptr(device=None) -> int:

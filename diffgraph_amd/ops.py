@@ -975,3 +975,76 @@ def nc_head_bwd(target, diff, w, ancs, label_out, entries, g_nll: torch.Tensor, 
                                     d_e.data_ptr(), d_row_loss.data_ptr(), d_w.data_ptr(), d_b.data_ptr(), _lib.stream_ptr(dev))
     _lib.check(rc, "dg_nc_head_bwd")
     return d_e, d_row_loss, d_w, d_b
+
+
+# --------------------------------------------------------------------------------------
+# embedding lookup
+# --------------------------------------------------------------------------------------
+_ELEMENT = {torch.float32: _lib.DG_F32, torch.bfloat16: _lib.DG_BF16, torch.float16: _lib.DG_F16}
+
+
+def _rows(x: torch.Tensor, name: str) -> torch.Tensor:
+    """A [rows, width] GPU tensor of one of the element types, the elements of a row next to each other."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype not in _ELEMENT or x.dim() != 2:
+        raise DiffGraphHipError(f"{name}: expected a 2-D float32, bfloat16 or float16 tensor on the GPU")
+    if x.shape[1] < 1:
+        raise DiffGraphHipError(f"{name}: rows have no columns")
+    if x.shape[1] > 1 and x.stride(1) != 1 or x.stride(0) < 0:
+        raise DiffGraphHipError(f"{name}: the elements of a row must lie next to each other (strides {tuple(x.stride())})")
+    return x
+
+
+def _ids(ids: torch.Tensor, device) -> torch.Tensor:
+    if not isinstance(ids, torch.Tensor) or ids.dtype not in (torch.int64, torch.int32) or ids.device != device:
+        raise DiffGraphHipError("ids: expected an int64 or int32 tensor on the table's GPU")
+    return ids if ids.is_contiguous() else ids.contiguous()
+
+
+def embedding_lookup(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """scale * table[ids] for table [rows, width] (float32 / bfloat16 / float16; rows may lie further apart than their
+    width) and int64 / int32 ids of any shape; [*ids.shape, width], rounded once.  An id outside the table: a row of NaN.
+    Not recorded by autograd: layers.embedding is."""
+    _rows(table, "table")
+    ids = _ids(ids, table.device)
+    n, dim = table.shape
+    if n < 1 and ids.numel():
+        raise DiffGraphHipError("table: has no rows to look up")
+    dev = table.device
+    with _lib.on_device(dev):
+        out = torch.empty((*ids.shape, dim), dtype=table.dtype, device=dev)
+        if out.numel():
+            rc = _lib.load().dg_embedding_lookup(table.data_ptr(), n, table.stride(0), dim, _ELEMENT[table.dtype], ids.data_ptr(),
+                                                 int(ids.dtype == torch.int64), ids.numel(), float(scale), out.data_ptr(),
+                                                 _lib.stream_ptr(dev))
+            _lib.check(rc, "dg_embedding_lookup")
+    return out
+
+
+def embedding_grad(d_out: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: float = 1.0,
+                   padding_idx: Optional[int] = None) -> torch.Tensor:
+    """The gradient of embedding_lookup's table, [n_rows, width] of d_out's type: per row, scale * the sum of the rows of
+    d_out [*ids.shape, width] whose id it is, in fp32 in the order of their positions (fixed chunks of the list sorted by
+    token: the same bits on every run); zeros where there are none.  Ids equal to padding_idx or outside [0, n_rows) take
+    no part."""
+    if not isinstance(d_out, torch.Tensor) or d_out.dim() < 1 or tuple(d_out.shape[:-1]) != tuple(ids.shape):
+        raise DiffGraphHipError(f"d_out: expected shape [*{tuple(ids.shape)}, width]")
+    if n_rows < 1:
+        raise DiffGraphHipError("n_rows: a table has at least one row")
+    dim, dev = d_out.shape[-1], d_out.device
+    d = d_out if d_out.dim() == 2 else d_out.reshape(-1, dim) if dim else d_out.reshape(0, 0)
+    if d.stride(1) != 1 or d.stride(0) < dim and d.shape[0] > 1:
+        d = d.contiguous()
+    _rows(d, "d_out")
+    ids = _ids(ids, dev)
+    if padding_idx is not None and not 0 <= padding_idx < n_rows:
+        raise DiffGraphHipError(f"padding_idx must lie in [0,{n_rows}); got {padding_idx}")
+    lib, n = _lib.load(), ids.numel()
+    with _lib.on_device(dev):
+        grad = torch.empty((n_rows, dim), dtype=d.dtype, device=dev)
+        ws_bytes = int(lib.dg_embedding_grad_workspace(n, n_rows, dim)) if n else 0
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        rc = lib.dg_embedding_grad(d.data_ptr(), d.stride(0), ids.data_ptr(), int(ids.dtype == torch.int64), n, n_rows, dim,
+                                   _ELEMENT[d.dtype], float(scale), -1 if padding_idx is None else int(padding_idx),
+                                   grad.data_ptr(), ws.data_ptr(), ws_bytes, _lib.stream_ptr(dev))
+        _lib.check(rc, "dg_embedding_grad")
+    return grad

@@ -690,6 +690,29 @@ int dg_spgemm_pattern_rows(const int32_t *a_rowptr, const int32_t *a_col, int32_
 int dg_spgemm_pattern_fill(const uint32_t *bitmap, int32_t n_rows, int32_t n_cols,
                            const int32_t *c_rowptr, int32_t *c_col, void *stream);
 
+/* ------------------------------------------------------------------------------------
+ * Embedding lookup with scaling and its gradient, for tables of any width: the batch gathers of
+ * DiffGraph-Rec/Model.py:101-105 (a, p, n = usr[ancs], itm[poss], itm[negs]) and what autograd forms for them.
+ *   dg_embedding_lookup   out[i][:] = scale * table[ids[i]][:]   (an id outside [0, n_rows): a row of NaN)
+ *   dg_embedding_grad     d_table[v][:] = scale * sum over { i : ids[i] = v } of d_out[i][:], the positions i in
+ *                         ascending order inside fixed chunks, in fp32, rounded once; EVERY row of d_table is
+ *                         written (zeros where no id names it), so it needs no clearing.  Ids outside [0, n_rows)
+ *                         and ids equal to padding_idx (-1: none) take no part.
+ * dtype: DG_F32 / DG_BF16 / DG_F16, for table, out, d_out and d_table alike.  row_stride: elements between the rows of
+ * table / d_out (out and d_table are contiguous).  ids: DEVICE int64 (ids_are_64 != 0) or int32.  At most 2^31 - 1 ids,
+ * 2^31 - 2 rows.  workspace: DEVICE, 16-byte aligned, dg_embedding_grad_workspace bytes, contents irrelevant; calls
+ * that may run at the same time need one each.
+ * ---------------------------------------------------------------------------------- */
+#define DG_F32 0
+#define DG_BF16 1
+#define DG_F16 2
+int dg_embedding_lookup(const void *table, int64_t n_rows, int64_t row_stride, int32_t dim, int32_t dtype,
+                        const void *ids, int32_t ids_are_64, int64_t n_ids, float scale, void *out, void *stream);
+size_t dg_embedding_grad_workspace(int64_t n_ids, int64_t n_rows, int32_t dim);
+int dg_embedding_grad(const void *d_out, int64_t row_stride, const void *ids, int32_t ids_are_64, int64_t n_ids,
+                      int64_t n_rows, int32_t dim, int32_t dtype, float scale, int64_t padding_idx, void *d_table,
+                      void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
