@@ -80,6 +80,16 @@ class WgradReduceTask(C.Structure):
                 ("d_w_out", C.c_void_p), ("d_b_out", C.c_void_p)]
 
 
+class ScoreTask(C.Structure):
+    _fields_ = [("scores", C.c_void_p), ("out", C.c_void_p), ("row_stride", C.c_int64), ("out_stride", C.c_int64),
+                ("n_rows", C.c_int32), ("n_items", C.c_int32), ("dtype", C.c_int32), ("exclude", C.c_int32),
+                ("hist_rowptr", C.c_void_p), ("hist_col", C.c_void_p), ("hist_rows", C.c_void_p), ("n_hist", C.c_int64),
+                ("n_hist_items", C.c_int64), ("repetition", C.c_void_p), ("frequency", C.c_void_p), ("presence", C.c_void_p),
+                ("repetition_all", C.c_float), ("frequency_all", C.c_float), ("presence_all", C.c_float), ("fill", C.c_float),
+                ("bias", C.c_void_p), ("bias_stride", C.c_int64), ("allowed", C.c_void_p), ("allowed_rows", C.c_void_p),
+                ("mask_words", C.c_int64), ("n_masks", C.c_int32)]
+
+
 # name -> (restype, argtypes); one entry per symbol declared in include/diffgraph_hip.h
 SIGNATURES = {
     "dg_version": (C.c_int, []),
@@ -178,6 +188,7 @@ SIGNATURES = {
     "dg_adam_multi": (C.c_int, [C.POINTER(C.c_void_p)] * 4 + [C.POINTER(C.c_int64), C.c_int32, C.c_void_p] + [C.c_float] * 5
                       + [C.c_void_p]),
     "dg_clear": (C.c_int, [C.c_void_p, C.c_size_t, C.c_void_p]),
+    "dg_adjust_scores": (C.c_int, [C.POINTER(ScoreTask), C.c_void_p]),
     "dg_embedding_lookup": (C.c_int, [C.c_void_p, C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_int32, C.c_int64,
                                       C.c_float, C.c_void_p, C.c_void_p]),
     "dg_embedding_grad_workspace": (C.c_size_t, [C.c_int64, C.c_int64, C.c_int32]),

@@ -44,3 +44,29 @@ __device__ __forceinline__ void dg_store(T *p, const float (&f)[VEC]) {
   for (int e = 0; e < VEC; ++e) w.v[e] = dg_round<T>(f[e]);
   *reinterpret_cast<dg_vec<T, VEC> *>(p) = w;
 }
+
+// The same for rows that start anywhere: the hardware takes vector accesses at any address of an element (a few more
+// cache lines touched), so only the ends of a row go element by element.
+template <int BYTES>
+struct dg_words {
+  typedef uint32_t type __attribute__((ext_vector_type(BYTES / 4), aligned(2)));
+};
+
+template <int VEC, typename T>
+__device__ __forceinline__ void dg_load_unaligned(const T *p, float (&f)[VEC]) {
+  const typename dg_words<sizeof(T) * VEC>::type q = *reinterpret_cast<const typename dg_words<sizeof(T) * VEC>::type *>(p);
+  T w[VEC];
+  __builtin_memcpy(w, &q, sizeof(w));
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) f[e] = dg_widen(w[e]);
+}
+
+template <int VEC, typename T>
+__device__ __forceinline__ void dg_store_unaligned(T *p, const float (&f)[VEC]) {
+  T w[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) w[e] = dg_round<T>(f[e]);
+  typename dg_words<sizeof(T) * VEC>::type q;
+  __builtin_memcpy(&q, w, sizeof(w));
+  *reinterpret_cast<typename dg_words<sizeof(T) * VEC>::type *>(p) = q;
+}

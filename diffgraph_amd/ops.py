@@ -1048,3 +1048,110 @@ def embedding_grad(d_out: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: f
                                    grad.data_ptr(), ws.data_ptr(), ws_bytes, _lib.stream_ptr(dev))
         _lib.check(rc, "dg_embedding_grad")
     return grad
+
+
+# --------------------------------------------------------------------------------------
+# scores
+# --------------------------------------------------------------------------------------
+def _on(x: torch.Tensor, name: str, dtype, device, dims) -> torch.Tensor:
+    if not isinstance(x, torch.Tensor) or x.dtype != dtype or x.device != device or x.dim() not in dims:
+        raise DiffGraphHipError(f"{name}: expected a {' or '.join(f'{d}-D' for d in dims)} {dtype} tensor on {device}")
+    return x
+
+
+def _per_row(v, name: str, n: int, device, neutral: float):
+    """(tensor or None, value for all rows) of a penalty given as a number, a float32 [n] tensor or None."""
+    if v is None:
+        return None, neutral
+    if isinstance(v, torch.Tensor):
+        _on(v, name, torch.float32, device, (1,))
+        if v.numel() != n:
+            raise DiffGraphHipError(f"{name}: expected one value for each of {n} rows, got {v.numel()}")
+        return v.contiguous(), neutral
+    return None, float(v)
+
+
+def adjust_scores(scores: torch.Tensor, *, history=None, rows: Optional[torch.Tensor] = None, repetition=None, frequency=None,
+                  presence=None, bias: Optional[torch.Tensor] = None, allowed: Optional[torch.Tensor] = None,
+                  allowed_rows: Optional[torch.Tensor] = None, exclude: bool = False, fill: float = -math.inf,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Penalties for items a row has had, a bias and masks on scores [rows, items] (float32 / bfloat16 / float16), in one pass:
+
+        s   = had ? (s > 0 ? s / repetition : s * repetition) - (frequency * had + presence) : s       had: the item's count
+        s   = s + bias[item]
+        out = (item not allowed, or exclude and had) ? fill : s
+
+    history: (rowptr, col), an int32 CSR of item ids, in any order, repeats counted; `rows` (int64 [rows]) names each score
+    row's line of it (default: its own number; a line that is not there is an empty history).  repetition (> 0), frequency,
+    presence: a number or float32 [rows].  bias: float32 [items] or [rows, items].  allowed: int32 words of 32 items, bit
+    v % 32 of word v // 32 set where item v stays, [words] for all rows or [masks, words] with allowed_rows (int32 [rows]; a
+    row whose number is not that of a mask has none; default: mask r for row r).  A row whose mask leaves nothing is all
+    `fill`.  out: where to (scores itself: in place)."""
+    _rows(scores, "scores")
+    n, items = scores.shape
+    dev = scores.device
+    if out is None:
+        out = torch.empty((n, items), dtype=scores.dtype, device=dev)
+    else:
+        _rows(out, "out")
+        if out.dtype != scores.dtype or out.shape != scores.shape or out.device != dev:
+            raise DiffGraphHipError("out: expected a tensor of scores' type, shape and device")
+        same = out.data_ptr() == scores.data_ptr() and out.stride() == scores.stride()
+        if not same and out.untyped_storage().data_ptr() == scores.untyped_storage().data_ptr():
+            raise DiffGraphHipError("out: must be scores itself or memory of its own")
+        if n > 1 and out.stride(0) < items:
+            raise DiffGraphHipError("out: its rows overlap")
+    t = _lib.ScoreTask()
+    t.scores, t.out, t.row_stride, t.out_stride = scores.data_ptr(), out.data_ptr(), scores.stride(0), out.stride(0)
+    t.n_rows, t.n_items, t.dtype, t.exclude, t.fill = n, items, _ELEMENT[scores.dtype], int(bool(exclude)), float(fill)
+    if history is not None:
+        rowptr, col = (_on(v, "history", torch.int32, dev, (1,)).contiguous() for v in history)
+        if rowptr.numel() < 1:
+            raise DiffGraphHipError("history: rowptr has one entry more than there are lines")
+        t.n_hist, t.n_hist_items = rowptr.numel() - 1, col.numel()
+        if rows is not None:
+            rows = _on(rows, "rows", torch.int64, dev, (1,)).contiguous()
+            if rows.numel() != n:
+                raise DiffGraphHipError(f"rows: expected one entry for each of {n} rows, got {rows.numel()}")
+            t.hist_rows = rows.data_ptr()
+        elif t.n_hist < n:
+            raise DiffGraphHipError(f"history: {t.n_hist} lines for {n} rows")
+        if col.numel():
+            t.hist_rowptr, t.hist_col = rowptr.data_ptr(), col.data_ptr()
+        else:
+            t.hist_rows = None
+    elif rows is not None or exclude or repetition is not None or frequency is not None or presence is not None:
+        raise DiffGraphHipError("history: penalties, rows and exclude need one")
+    rep, t.repetition_all = _per_row(repetition, "repetition", n, dev, 1.0)
+    fre, t.frequency_all = _per_row(frequency, "frequency", n, dev, 0.0)
+    pre, t.presence_all = _per_row(presence, "presence", n, dev, 0.0)
+    if not t.repetition_all > 0:
+        raise DiffGraphHipError(f"repetition must be positive, got {t.repetition_all}")
+    t.repetition, t.frequency, t.presence = _ptr(rep), _ptr(fre), _ptr(pre)
+    if bias is not None:
+        _on(bias, "bias", torch.float32, dev, (1, 2))
+        if bias.shape[-1] != items or (bias.dim() == 2 and bias.shape[0] != n):
+            raise DiffGraphHipError(f"bias: expected shape [{items}] or [{n}, {items}], got {tuple(bias.shape)}")
+        if items > 1 and bias.stride(-1) != 1 or bias.stride(0) < 0:
+            bias = bias.contiguous()
+        t.bias, t.bias_stride = bias.data_ptr(), bias.stride(0) if bias.dim() == 2 else 0
+    if allowed is not None:
+        allowed = _on(allowed, "allowed", torch.int32, dev, (1, 2)).contiguous()
+        if allowed.shape[-1] < (items + 31) // 32:
+            raise DiffGraphHipError(f"allowed: {(items + 31) // 32} words hold {items} items, got {allowed.shape[-1]}")
+        masks = allowed.shape[0] if allowed.dim() == 2 else 1
+        if allowed_rows is not None:
+            allowed_rows = _on(allowed_rows, "allowed_rows", torch.int32, dev, (1,)).contiguous()
+            if allowed_rows.numel() != n:
+                raise DiffGraphHipError(f"allowed_rows: expected one entry for each of {n} rows, got {allowed_rows.numel()}")
+        elif masks not in (1, n):
+            raise DiffGraphHipError(f"allowed: {masks} masks for {n} rows: allowed_rows says which")
+        if masks < 1:
+            raise DiffGraphHipError("allowed: no mask given")
+        t.allowed, t.allowed_rows, t.mask_words, t.n_masks = allowed.data_ptr(), _ptr(allowed_rows), allowed.shape[-1], masks
+    elif allowed_rows is not None:
+        raise DiffGraphHipError("allowed: allowed_rows needs masks")
+    if n and items:
+        with _lib.on_device(dev):
+            _lib.check(_lib.load().dg_adjust_scores(C.byref(t), _lib.stream_ptr(dev)), "dg_adjust_scores")
+    return out

@@ -713,6 +713,44 @@ int dg_embedding_grad(const void *d_out, int64_t row_stride, const void *ids, in
                       int64_t n_rows, int32_t dim, int32_t dtype, float scale, int64_t padding_idx, void *d_table,
                       void *workspace, size_t workspace_bytes, void *stream);
 
+/* ------------------------------------------------------------------------------------
+ * Penalties, biases and masks on scores [n_rows][n_items], between t.mm(usr, itm^T) and t.topk of
+ * DiffGraph-Rec/main.py:157-158 (whose mask of training items is `exclude` with fill = -1e8).  Per row and item,
+ * with had = how often the item occurs in the row's history:
+ *   s   = had ? (s > 0 ? s / repetition : s * repetition) - (frequency * had + presence) : s
+ *   s   = s + bias[item]
+ *   out = (item not in the row's mask, or exclude and had) ? fill : s
+ * in fp32, rounded once (a fill beyond the type's range becomes an infinity).  What masked places hold does not matter;
+ * a row whose mask leaves nothing is all fill.
+ *   scores, out       DEVICE, dtype DG_F32 / DG_BF16 / DG_F16, rows row_stride / out_stride elements apart; out may be
+ *                     scores (same stride), and must not overlap it otherwise
+ *   hist_rowptr, hist_col   DEVICE int32 CSR of n_hist rows and n_hist_items entries, any order, repeats counted (NULL:
+ *                     no history); ids outside [0, n_items) are passed over.  hist_rows: DEVICE int64[n_rows], the CSR
+ *                     row of a score row (NULL: its own number; outside [0, n_hist): no history)
+ *   repetition, frequency, presence   DEVICE float[n_rows], or NULL: the value *_all for every row
+ *   bias              DEVICE float, item v of row r at bias[r * bias_stride + v] (bias_stride 0: one for all rows)
+ *   allowed           DEVICE uint32[n_masks][mask_words], bit v & 31 of word v >> 5 set: item v stays.  allowed_rows:
+ *                     DEVICE int32[n_rows], a row's mask (outside [0, n_masks): none); NULL: mask 0 of one, else its own
+ * ---------------------------------------------------------------------------------- */
+typedef struct {
+  const void *scores;
+  void *out;
+  int64_t row_stride, out_stride;
+  int32_t n_rows, n_items, dtype, exclude;
+  const int32_t *hist_rowptr, *hist_col;
+  const int64_t *hist_rows;
+  int64_t n_hist, n_hist_items;
+  const float *repetition, *frequency, *presence;
+  float repetition_all, frequency_all, presence_all, fill;
+  const float *bias;
+  int64_t bias_stride;
+  const uint32_t *allowed;
+  const int32_t *allowed_rows;
+  int64_t mask_words;
+  int32_t n_masks;
+} dg_score_task;
+int dg_adjust_scores(const dg_score_task *task, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
