@@ -13,7 +13,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libdiffgraph_hip.so")
 SOURCES = ["graph.hip", "spmm.hip", "fused.hip", "diffusion.hip", "wgrad.hip", "losshead.hip", "eval.hip", "sampling.hip", "spgemm.hip", "optim.hip", "linear.hip", "comm.hip",
-           "embedding.hip", "scores.hip"]
+           "embedding.hip", "scores.hip", "checkpoint8.hip"]
 HEADERS = [os.path.join(CSRC, "dg_internal.h"), os.path.join(CSRC, "dg_gather.h"), os.path.join(CSRC, "dg_philox.h"), os.path.join(CSRC, "dg_wgrad.h"), os.path.join(CSRC, "dg_types.h"), os.path.join(HERE, "..", "include", "diffgraph_hip.h")]
 # (no packed fp32 instructions: some forms the compiler picks by itself have given wrong results on this hardware)
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Wall", "-Wno-unused-function",

@@ -1,0 +1,521 @@
+// Activation checkpoints in 8 bits and the backward pass of a dense layer out of them, for gfx950.
+//
+// Kept of x [n][k]: one byte per element and one scale per group of 32 columns of a row, the smallest power of two with
+// (largest of the group) <= 127 scale (int8) or 448 scale (e4m3), so that no code saturates and the codes' values,
+//   x^ = code * scale,   code = x / scale rounded to the nearest code (ties to even),
+// are exact in bf16: at most seven (int8) or four (e4m3) significant bits.  A group that holds an infinity or a NaN stands
+// for NaN as a whole.
+//
+// The layer's backward (nn.Linear with tanh behind it: DiffGraph-Rec/Model.py:228-233) out of the codes of its input x
+// and, with tanh, of its output y:
+//   d_z = d_y (1 - y^ y^)      d_w = d_z^T . x^      d_b = column sums of d_z
+// The product runs on the bf16 matrix instruction: x^ is exact there, and d_z (fp32) is cut into bf16 numbers that add up
+// to it -- three for fp32 (all 24 bits), two for fp16 and for d_z formed from bf16 (16 bits, beyond what the 16-bit result
+// shows), one for bf16 as it came -- with sums in fp32.  Rows are cut into strips whose partial results a second launch
+// adds in strip order: the same bits on every run.
+#include "dg_internal.h"
+#include "dg_types.h"
+
+namespace {
+
+constexpr int kGroup = 32, kLowest = -110;      // columns per scale; smallest exponent (code values stay normal in bf16)
+constexpr uint32_t kNoNumber = 255;             // scale byte of a group that stands for NaN
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// ---- codes ------------------------------------------------------------------------------------------------------
+// Scale byte (exponent + 127) of a group whose largest magnitude has the bits `top`.
+template <int FMT>
+__device__ __forceinline__ uint32_t scale_byte(uint32_t top) {
+  if (top >= 0x7f800000u) return kNoNumber;
+  const int e = (int)(top >> 23) - 127;                                  // top = (1 + m / 2^23) 2^e
+  const uint32_t m = top & 0x7fffffu;
+  const int s = FMT == DG_E4M3 ? e - 8 + (m > 0x600000u)                 // 448 = 1.75 * 2^8
+                               : e - 6 + (m > 0x7e0000u);                // 127 = 1.984375 * 2^6
+  return (uint32_t)(max(s, kLowest) + 127);
+}
+
+template <int FMT>
+__device__ __forceinline__ uint32_t encode4(const float *q) {
+  if constexpr (FMT == DG_E4M3) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], w, true);
+  } else {
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w |= ((uint32_t)(int)rintf(q[e]) & 255u) << (8 * e);
+    return w;
+  }
+}
+
+// The four codes' values; a scale byte is the exponent field of its fp32 value (255: infinity, times code 0 = NaN).
+template <int FMT>
+__device__ __forceinline__ void decode4(uint32_t w, uint32_t byte, float (&f)[4]) {
+  const float s = __uint_as_float(byte << 23);
+  if constexpr (FMT == DG_E4M3) {
+    const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+    f[0] = a[0] * s; f[1] = a[1] * s; f[2] = b[0] * s; f[3] = b[1] * s;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = (float)(int8_t)(w >> (8 * e)) * s;
+  }
+}
+
+// Four neighbouring lanes take a group, eight columns each; a row takes `lanes` = 4 ceil(k / 32) of them.
+template <typename T, int FMT>
+__global__ __launch_bounds__(256) void checkpoint8_kernel(const T *__restrict__ x, int64_t stride, int64_t n, int k, int pitch,
+                                                          int lanes, int rows_per_block, uint8_t *__restrict__ codes,
+                                                          uint8_t *__restrict__ scales) {
+  const int r = threadIdx.x / min(lanes, 256);
+  const int64_t row = (int64_t)blockIdx.x * rows_per_block + r;
+  if (r >= rows_per_block || row >= n) return;
+  for (int u = threadIdx.x - r * min(lanes, 256); u < lanes; u += 256) {
+    const int c = u * 8;
+    float f[8];
+    if (c + 8 <= k) {
+      dg_load_unaligned<8>(x + row * stride + c, f);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = c + e < k ? dg_widen(x[row * stride + c + e]) : 0.f;
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
+    top = max(top, (uint32_t)__shfl_xor((int)top, 1));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 2));
+    const uint32_t byte = scale_byte<FMT>(top);
+    const float inv = byte == kNoNumber ? 0.f : __uint_as_float((254u - byte) << 23);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = byte == kNoNumber ? 0.f : f[e] * inv;
+    if (c < pitch) {
+      const u32x2 w = {encode4<FMT>(f), encode4<FMT>(f + 4)};
+      *reinterpret_cast<u32x2 *>(codes + row * pitch + c) = w;
+    }
+    if ((u & 3) == 0) scales[row * (lanes >> 2) + (u >> 2)] = (uint8_t)byte;
+  }
+}
+
+template <typename T, int FMT>
+__global__ __launch_bounds__(256) void checkpoint8_values_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales,
+                                                                 int64_t n, int k, int pitch, int lanes, int rows_per_block,
+                                                                 T *__restrict__ out) {
+  const int r = threadIdx.x / min(lanes, 256);
+  const int64_t row = (int64_t)blockIdx.x * rows_per_block + r;
+  if (r >= rows_per_block || row >= n) return;
+  for (int u = threadIdx.x - r * min(lanes, 256); u < lanes; u += 256) {
+    const int c = u * 8;
+    if (c >= k) continue;
+    const u32x2 w = *reinterpret_cast<const u32x2 *>(codes + row * pitch + c);
+    const uint32_t byte = scales[row * (lanes >> 2) + (u >> 2)];
+    float lo[4], hi[4];
+    decode4<FMT>(w[0], byte, lo);
+    decode4<FMT>(w[1], byte, hi);
+    const float f[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    T *dst = out + row * k + c;
+    if (c + 8 <= k) {
+      dg_store_unaligned<8>(dst, f);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (c + e < k) dst[e] = dg_round<T>(f[e]);
+    }
+  }
+}
+
+// ---- the layer's backward -----------------------------------------------------------------------------------------
+struct back_args {
+  const void *d_y;
+  int64_t d_stride;
+  const uint8_t *x, *x_scales, *y, *y_scales;
+  int x_pitch, x_groups, y_pitch, y_groups;
+  int64_t n;
+  int k, m;
+  int64_t rows_per_strip;
+  int strips, tiles_m, tiles_n;
+  void *d_z;            // contiguous [n][m], written under tanh
+  float *part, *part_b; // [strip][tile_m][tile_n][BM][BN], [strip][tiles_m * BM]
+};
+
+__device__ __forceinline__ uint32_t high_halves(float a, float b) {   // bf16(a) | bf16(b) << 16, by truncation
+  return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
+
+// A workgroup sums one strip of rows for a BM x BN tile of d_w, BK rows at a time: its threads load quads of rows x quads
+// of columns, form d_z, cut it, and lay both operands down in LDS with eight rows of a column in 16 bytes -- what a lane
+// of the matrix instruction takes -- transposing in their registers.  A column c sits in slot (c mod 4) (B / 4) + c / 4, so
+// that neighbouring lanes write neighbouring slots; results are kept in slot order until the second launch.
+// The next rows are on their way while the matrix instructions run.
+template <typename T, int FMT, bool TANH, int PIECES, int BM, int BN>
+__global__ __launch_bounds__(256) void checkpoint8_backward_kernel(back_args a) {
+  constexpr int BK = BM == 128 && BN == 128 ? 32 : 64, WM = BM / 2, WN = BN / 2, TM = WM / 32, TN = WN / 32;
+  constexpr int UA = BM * BK / 16 / 256, UB = BN * BK / 16 / 256;      // 4 x 4 units per thread and step
+  __shared__ u32x4 lds_a[PIECES][BK / 8][BM], lds_b[BK / 8][BN];
+  __shared__ float col_sums[BK / 4][BM];
+  const int tiles = a.tiles_m * a.tiles_n;
+  const int xcd = blockIdx.x & 7, idx = blockIdx.x >> 3;               // the tiles of a strip share an L2
+  const int strip = idx / tiles * 8 + xcd, tile = idx % tiles;
+  if (strip >= a.strips) return;
+  const int m0 = tile / a.tiles_n * BM, n0 = tile % a.tiles_n * BN;
+  const bool first_n = n0 == 0;
+  const int64_t r0 = (int64_t)strip * a.rows_per_strip, r1 = min(r0 + a.rows_per_strip, a.n);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = (wave >> 1) * WM, wn = (wave & 1) * WN;
+
+  float d[UA][4][4];
+  uint32_t yw[UA][4], ys[UA][4], xw[UB][4], xs[UB][4];
+  float sums[UA][4];
+#pragma unroll
+  for (int u = 0; u < UA; ++u)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sums[u][j] = 0.f;
+  f32x16 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+
+  auto fetch = [&](int64_t base) {
+#pragma unroll
+    for (int u = 0; u < UA; ++u) {
+      const int unit = tid + 256 * u, c = m0 + unit % (BM / 4) * 4;
+      const int64_t row = base + unit / (BM / 4) * 4;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const bool in = row + q < r1 && c < a.m;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) d[u][q][j] = 0.f;
+        if (TANH) yw[u][q] = ys[u][q] = 0;
+        if (!in) continue;
+        const T *src = (const T *)a.d_y + (row + q) * a.d_stride + c;
+        if (c + 4 <= a.m) {
+          dg_load_unaligned<4>(src, d[u][q]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (c + j < a.m) d[u][q][j] = dg_widen(src[j]);
+        }
+        if (TANH) {
+          yw[u][q] = *reinterpret_cast<const uint32_t *>(a.y + (row + q) * a.y_pitch + c);
+          ys[u][q] = a.y_scales[(row + q) * a.y_groups + c / kGroup];
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < UB; ++u) {
+      const int unit = tid + 256 * u, c = n0 + unit % (BN / 4) * 4;
+      const int64_t row = base + unit / (BN / 4) * 4;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        xw[u][q] = xs[u][q] = 0;
+        if (row + q < r1 && c < a.k) {
+          xw[u][q] = *reinterpret_cast<const uint32_t *>(a.x + (row + q) * a.x_pitch + c);
+          xs[u][q] = a.x_scales[(row + q) * a.x_groups + c / kGroup];
+        }
+      }
+    }
+  };
+
+  auto lay_down = [&](int64_t base) {
+#pragma unroll
+    for (int u = 0; u < UA; ++u) {
+      const int unit = tid + 256 * u, c4 = unit % (BM / 4), rq = unit / (BM / 4), c = m0 + c4 * 4;
+      if (TANH) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float y[4];
+          decode4<FMT>(yw[u][q], ys[u][q], y);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) d[u][q][j] *= 1.f - y[j] * y[j];
+          const int64_t row = base + rq * 4 + q;
+          if (first_n && row < r1 && c < a.m) {
+            T *dst = (T *)a.d_z + row * a.m + c;
+            if (c + 4 <= a.m) {
+              dg_store_unaligned<4>(dst, d[u][q]);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (c + j < a.m) dst[j] = dg_round<T>(d[u][q][j]);
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = d[u][q][j];
+        sums[u][j] += (v[0] + v[1]) + (v[2] + v[3]);
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+          const u32x2 w = {high_halves(v[0], v[1]), high_halves(v[2], v[3])};
+          reinterpret_cast<u32x2 *>(&lds_a[p][rq >> 1][j * (BM / 4) + c4])[rq & 1] = w;
+          if (p + 1 < PIECES) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] -= __uint_as_float(__float_as_uint(v[q]) & 0xffff0000u);   // (exact)
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < UB; ++u) {
+      const int unit = tid + 256 * u, c4 = unit % (BN / 4), rq = unit / (BN / 4);
+      float v[4][4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) decode4<FMT>(xw[u][q], xs[u][q], v[q]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const u32x2 w = {high_halves(v[0][j], v[1][j]), high_halves(v[2][j], v[3][j])};
+        reinterpret_cast<u32x2 *>(&lds_b[rq >> 1][j * (BN / 4) + c4])[rq & 1] = w;
+      }
+    }
+  };
+
+  fetch(r0);
+  for (int64_t base = r0; base < r1; base += BK) {
+    lay_down(base);
+    __syncthreads();
+    if (base + BK < r1) fetch(base + BK);
+#pragma unroll
+    for (int kk = 0; kk < BK / 16; ++kk) {
+      const int k8 = kk * 2 + (lane >> 5);
+      bf16x8 fb[TN];
+#pragma unroll
+      for (int j = 0; j < TN; ++j) fb[j] = __builtin_bit_cast(bf16x8, lds_b[k8][wn + j * 32 + (lane & 31)]);
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p)
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          const bf16x8 fa = __builtin_bit_cast(bf16x8, lds_a[p][k8][wm + i * 32 + (lane & 31)]);
+#pragma unroll
+          for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa, fb[j], acc[i][j], 0, 0, 0);
+        }
+    }
+    __syncthreads();
+  }
+
+  float *part = a.part + ((size_t)strip * tiles + tile) * (BM * BN);
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        part[(size_t)(wm + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * BN + wn + j * 32 + (lane & 31)] = acc[i][j][e];
+  if (!first_n) return;
+#pragma unroll
+  for (int u = 0; u < UA; ++u) {
+    const int unit = tid + 256 * u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) col_sums[unit / (BM / 4)][unit % (BM / 4) * 4 + j] = sums[u][j];
+  }
+  __syncthreads();
+  for (int c = tid; c < BM; c += 256) {
+    float s = 0.f;
+    for (int q = 0; q < BK / 4; ++q) s += col_sums[q][c];
+    a.part_b[(size_t)strip * (a.tiles_m * BM) + m0 + c] = s;
+  }
+}
+
+// Adds the strips' parts, 16 strands of every 16th strip each, the strands in order.  A block takes 64 neighbouring
+// values: of a tile (in slot order), or -- the blocks behind them -- of the column sums.
+template <typename T, int BM, int BN>
+__global__ __launch_bounds__(256) void checkpoint8_reduce_kernel(const float *__restrict__ part, const float *__restrict__ part_b,
+                                                                 int strips, int tiles_m, int tiles_n, int m, int k,
+                                                                 T *__restrict__ d_w, T *__restrict__ d_b) {
+  __shared__ float strand[16][64];
+  const int tiles = tiles_m * tiles_n, blocks_w = tiles * (BM * BN / 64);
+  const bool bias = (int)blockIdx.x >= blocks_w;
+  const size_t at = bias ? (size_t)(blockIdx.x - blocks_w) * 64 : (size_t)blockIdx.x * 64;
+  const size_t step = bias ? (size_t)tiles_m * BM : (size_t)tiles * BM * BN;
+  const float *src = (bias ? part_b : part) + at;
+  const int g = threadIdx.x >> 4, l = threadIdx.x & 15;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s = g; s < strips; s += 16) {
+    float f[4];
+    dg_load<4>(src + s * step + 4 * l, f);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] += f[e];
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) strand[g][4 * l + e] = acc[e];
+  __syncthreads();
+  if (threadIdx.x >= 64) return;
+  float s = strand[0][threadIdx.x];
+  for (int q = 1; q < 16; ++q) s += strand[q][threadIdx.x];
+  if (bias) {
+    const size_t o = at + threadIdx.x;
+    if (o < (size_t)m) d_b[o] = dg_round<T>(s);
+    return;
+  }
+  const int tile = (int)(at / (BM * BN)), in = (int)(at % (BM * BN)) + threadIdx.x, i = in / BN, j = in % BN;
+  const int o = tile / tiles_n * BM + i % (BM / 4) * 4 + i / (BM / 4), c = tile % tiles_n * BN + j % (BN / 4) * 4 + j / (BN / 4);
+  if (o < m && c < k) d_w[(size_t)o * k + c] = dg_round<T>(s);
+}
+
+// ---- host side --------------------------------------------------------------------------------------------------
+int type_size(int dtype) { return dtype == DG_F32 ? 4 : (dtype == DG_BF16 || dtype == DG_F16) ? 2 : 0; }
+int pitch_of(int k) { return (k + 15) / 16 * 16; }
+int groups_of(int k) { return (k + kGroup - 1) / kGroup; }
+
+int check_sizes(const char *what, int64_t n, int64_t k, int fmt) {
+  if (fmt != DG_INT8 && fmt != DG_E4M3) return dg_fail(DG_ERR_ARG, "%s: unknown 8-bit format %d", what, fmt);
+  if (n < 0 || k <= 0) return dg_fail(DG_ERR_ARG, "%s: bad sizes", what);
+  if (k > (1 << 20) || n > 0x7fffffff) return dg_fail(DG_ERR_SIZE, "%s: at most 2^31 - 1 rows of 2^20 columns", what);
+  return 0;
+}
+
+struct row_grid {
+  int lanes, rows_per_block;
+  unsigned blocks;
+};
+row_grid rows_of(int64_t n, int k) {
+  row_grid g;
+  g.lanes = 4 * groups_of(k);
+  g.rows_per_block = g.lanes >= 256 ? 1 : 256 / g.lanes;
+  g.blocks = (unsigned)((n + g.rows_per_block - 1) / g.rows_per_block);
+  return g;
+}
+
+// Tiles of 128 where that many columns are there; strips so that some 512 workgroups run, of at least 256 rows each.
+struct back_plan {
+  int bm, bn, tiles_m, tiles_n, strips;
+  int64_t rows_per_strip;
+  size_t part, part_b, bytes;
+};
+back_plan plan_of(int64_t n, int k, int m) {
+  back_plan p;
+  p.bm = m > 64 ? 128 : 64;
+  p.bn = k > 64 ? 128 : 64;
+  p.tiles_m = (m + p.bm - 1) / p.bm;
+  p.tiles_n = (k + p.bn - 1) / p.bn;
+  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
+  int64_t strips = (512 + tiles - 1) / tiles;
+  strips = strips < (n + 255) / 256 ? strips : (n + 255) / 256;
+  p.rows_per_strip = strips ? ((n + strips - 1) / strips + 63) / 64 * 64 : 64;
+  p.strips = (int)((n + p.rows_per_strip - 1) / p.rows_per_strip);
+  p.part = 0;
+  p.part_b = (size_t)p.strips * tiles * p.bm * p.bn * 4;
+  p.bytes = p.part_b + (size_t)p.strips * p.tiles_m * p.bm * 4 + 256;
+  return p;
+}
+
+template <typename T, int FMT, bool TANH, int PIECES, int BM, int BN>
+int back_as(const back_plan &p, const back_args &a, T *d_w, T *d_b, hipStream_t stream) {
+  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, blocks = (int64_t)(p.strips + 7) / 8 * 8 * tiles;
+  if (blocks > 0x7fffffff || tiles * (BM * BN / 64) + p.tiles_m * (BM / 64) > 0x7fffffff)
+    return dg_fail(DG_ERR_SIZE, "dg_checkpoint8_backward: a weight of %d x %d is too large", a.m, a.k);
+  if (p.strips) {
+    hipLaunchKernelGGL((checkpoint8_backward_kernel<T, FMT, TANH, PIECES, BM, BN>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
+    DG_HIP(hipGetLastError());
+  }
+  hipLaunchKernelGGL((checkpoint8_reduce_kernel<T, BM, BN>), dim3((unsigned)(tiles * (BM * BN / 64) + p.tiles_m * (BM / 64))), dim3(256), 0,
+                     stream, a.part, a.part_b, p.strips, p.tiles_m, p.tiles_n, a.m, a.k, d_w, d_b);
+  DG_HIP(hipGetLastError());
+  return 0;
+}
+
+template <typename T, int FMT, bool TANH, int PIECES>
+int back_tiles(const back_plan &p, const back_args &a, void *d_w, void *d_b, hipStream_t stream) {
+  if (p.bm == 128) {
+    if (p.bn == 128) return back_as<T, FMT, TANH, PIECES, 128, 128>(p, a, (T *)d_w, (T *)d_b, stream);
+    return back_as<T, FMT, TANH, PIECES, 128, 64>(p, a, (T *)d_w, (T *)d_b, stream);
+  }
+  if (p.bn == 128) return back_as<T, FMT, TANH, PIECES, 64, 128>(p, a, (T *)d_w, (T *)d_b, stream);
+  return back_as<T, FMT, TANH, PIECES, 64, 64>(p, a, (T *)d_w, (T *)d_b, stream);
+}
+
+template <typename T, int PLAIN, int WITH_TANH>
+int back_forms(int fmt, bool tanh, const back_plan &p, const back_args &a, void *d_w, void *d_b, hipStream_t stream) {
+  if (fmt == DG_E4M3)
+    return tanh ? back_tiles<T, DG_E4M3, true, WITH_TANH>(p, a, d_w, d_b, stream) : back_tiles<T, DG_E4M3, false, PLAIN>(p, a, d_w, d_b, stream);
+  return tanh ? back_tiles<T, DG_INT8, true, WITH_TANH>(p, a, d_w, d_b, stream) : back_tiles<T, DG_INT8, false, PLAIN>(p, a, d_w, d_b, stream);
+}
+
+}  // namespace
+
+extern "C" int32_t dg_checkpoint8_pitch(int32_t k) { return k > 0 && k <= (1 << 20) ? pitch_of(k) : 0; }
+extern "C" int32_t dg_checkpoint8_groups(int32_t k) { return k > 0 && k <= (1 << 20) ? groups_of(k) : 0; }
+
+extern "C" int dg_checkpoint8(const void *x, int64_t row_stride, int64_t n, int32_t k, int32_t dtype, int32_t format, void *codes,
+                              void *scales, void *stream) {
+  if (const int rc = check_sizes("dg_checkpoint8", n, k, format)) return rc;
+  if (!type_size(dtype)) return dg_fail(DG_ERR_ARG, "dg_checkpoint8: unknown element type %d", dtype);
+  if (row_stride < 0) return dg_fail(DG_ERR_ARG, "dg_checkpoint8: negative row stride");
+  if (n == 0) return 0;
+  if (!x || !codes || !scales) return dg_fail(DG_ERR_ARG, "dg_checkpoint8: NULL argument");
+  if ((uintptr_t)codes & 15) return dg_fail(DG_ERR_ARG, "dg_checkpoint8: codes must be 16-byte aligned");
+  const row_grid g = rows_of(n, k);
+#define DG_KEEP(T, F)                                                                                                       \
+  hipLaunchKernelGGL((checkpoint8_kernel<T, F>), dim3(g.blocks), dim3(256), 0, (hipStream_t)stream, (const T *)x, row_stride, n, k, \
+                     pitch_of(k), g.lanes, g.rows_per_block, (uint8_t *)codes, (uint8_t *)scales)
+  if (format == DG_E4M3) {
+    if (dtype == DG_F32) DG_KEEP(float, DG_E4M3);
+    else if (dtype == DG_BF16) DG_KEEP(dg_bf16, DG_E4M3);
+    else DG_KEEP(dg_f16, DG_E4M3);
+  } else {
+    if (dtype == DG_F32) DG_KEEP(float, DG_INT8);
+    else if (dtype == DG_BF16) DG_KEEP(dg_bf16, DG_INT8);
+    else DG_KEEP(dg_f16, DG_INT8);
+  }
+#undef DG_KEEP
+  DG_HIP(hipGetLastError());
+  return 0;
+}
+
+extern "C" int dg_checkpoint8_values(const void *codes, const void *scales, int64_t n, int32_t k, int32_t format, int32_t dtype, void *out,
+                                     void *stream) {
+  if (const int rc = check_sizes("dg_checkpoint8_values", n, k, format)) return rc;
+  if (!type_size(dtype)) return dg_fail(DG_ERR_ARG, "dg_checkpoint8_values: unknown element type %d", dtype);
+  if (n == 0) return 0;
+  if (!codes || !scales || !out) return dg_fail(DG_ERR_ARG, "dg_checkpoint8_values: NULL argument");
+  if ((uintptr_t)codes & 15) return dg_fail(DG_ERR_ARG, "dg_checkpoint8_values: codes must be 16-byte aligned");
+  const row_grid g = rows_of(n, k);
+#define DG_READ(T, F)                                                                                                            \
+  hipLaunchKernelGGL((checkpoint8_values_kernel<T, F>), dim3(g.blocks), dim3(256), 0, (hipStream_t)stream, (const uint8_t *)codes, \
+                     (const uint8_t *)scales, n, k, pitch_of(k), g.lanes, g.rows_per_block, (T *)out)
+  if (format == DG_E4M3) {
+    if (dtype == DG_F32) DG_READ(float, DG_E4M3);
+    else if (dtype == DG_BF16) DG_READ(dg_bf16, DG_E4M3);
+    else DG_READ(dg_f16, DG_E4M3);
+  } else {
+    if (dtype == DG_F32) DG_READ(float, DG_INT8);
+    else if (dtype == DG_BF16) DG_READ(dg_bf16, DG_INT8);
+    else DG_READ(dg_f16, DG_INT8);
+  }
+#undef DG_READ
+  DG_HIP(hipGetLastError());
+  return 0;
+}
+
+extern "C" size_t dg_checkpoint8_backward_workspace(int64_t n, int32_t k, int32_t m) {
+  if (n < 0 || k <= 0 || m <= 0 || n > 0x7fffffff || k > (1 << 20) || m > (1 << 20)) return 0;
+  return plan_of(n, k, m).bytes;
+}
+
+extern "C" int dg_checkpoint8_backward(const void *d_y, int64_t row_stride, int64_t n, int32_t m, int32_t k, int32_t dtype, int32_t format,
+                                       const void *x_codes, const void *x_scales, const void *y_codes, const void *y_scales, void *d_z,
+                                       void *d_w, void *d_b, void *workspace, size_t workspace_bytes, void *stream) {
+  if (const int rc = check_sizes("dg_checkpoint8_backward", n, k, format)) return rc;
+  if (const int rc = check_sizes("dg_checkpoint8_backward", n, m, format)) return rc;
+  if (!type_size(dtype)) return dg_fail(DG_ERR_ARG, "dg_checkpoint8_backward: unknown element type %d", dtype);
+  if (row_stride < 0) return dg_fail(DG_ERR_ARG, "dg_checkpoint8_backward: negative row stride");
+  const bool tanh = y_codes != nullptr;
+  if (!d_w || !d_b || !workspace || (n && (!d_y || !x_codes || !x_scales || (tanh && (!y_scales || !d_z)))))
+    return dg_fail(DG_ERR_ARG, "dg_checkpoint8_backward: NULL argument");
+  if (((uintptr_t)x_codes | (uintptr_t)y_codes | (uintptr_t)workspace) & 15)
+    return dg_fail(DG_ERR_ARG, "dg_checkpoint8_backward: codes and workspace must be 16-byte aligned");
+  const back_plan p = plan_of(n, k, m);
+  if (workspace_bytes < p.bytes)
+    return dg_fail(DG_ERR_SIZE, "dg_checkpoint8_backward: workspace of %zu bytes, %zu needed", workspace_bytes, p.bytes);
+  back_args a = {d_y, row_stride, (const uint8_t *)x_codes, (const uint8_t *)x_scales, (const uint8_t *)y_codes, (const uint8_t *)y_scales,
+                 pitch_of(k), groups_of(k), pitch_of(m), groups_of(m), n, k, m, p.rows_per_strip, p.strips, p.tiles_m, p.tiles_n, d_z,
+                 (float *)workspace, (float *)((char *)workspace + p.part_b)};
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == DG_F32) return back_forms<float, 3, 3>(format, tanh, p, a, d_w, d_b, st);
+  if (dtype == DG_BF16) return back_forms<dg_bf16, 1, 2>(format, tanh, p, a, d_w, d_b, st);
+  return back_forms<dg_f16, 2, 2>(format, tanh, p, a, d_w, d_b, st);
+}

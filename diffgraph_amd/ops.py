@@ -1155,3 +1155,87 @@ def adjust_scores(scores: torch.Tensor, *, history=None, rows: Optional[torch.Te
         with _lib.on_device(dev):
             _lib.check(_lib.load().dg_adjust_scores(C.byref(t), _lib.stream_ptr(dev)), "dg_adjust_scores")
     return out
+
+
+# --------------------------------------------------------------------------------------
+# activation checkpoints in 8 bits
+# --------------------------------------------------------------------------------------
+_FORMATS = {"int8": _lib.DG_INT8, "e4m3": _lib.DG_E4M3}
+
+
+@dataclass
+class Checkpoint8:
+    """What is kept of an activation [n, k]: one code byte per element and one scale byte per 32 columns of a row
+    (checkpoint8).  A group that held an infinity or a NaN stands for NaN as a whole."""
+    codes: torch.Tensor         # uint8 [n, k rounded up to 16]
+    scales: torch.Tensor        # uint8 [n, ceil(k / 32)]: exponent + 127, 255 = NaN
+    shape: tuple
+    format: str
+
+    def values(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The [n, k] values the codes stand for (exact in float32 and bfloat16)."""
+        if dtype not in _ELEMENT:
+            raise DiffGraphHipError(f"values: float32, bfloat16 or float16, not {dtype}")
+        n, k = self.shape
+        dev = self.codes.device
+        with _lib.on_device(dev):
+            out = torch.empty((n, k), dtype=dtype, device=dev)
+            rc = _lib.load().dg_checkpoint8_values(self.codes.data_ptr(), self.scales.data_ptr(), n, k, _FORMATS[self.format],
+                                                   _ELEMENT[dtype], out.data_ptr(), _lib.stream_ptr(dev))
+            _lib.check(rc, "dg_checkpoint8_values")
+        return out
+
+    def check(self, name: str, n: int, device) -> None:
+        if not isinstance(self, Checkpoint8):
+            raise DiffGraphHipError(f"{name}: expected what checkpoint8 returns")
+        k = self.shape[1]
+        for t, w in ((self.codes, (k + 15) // 16 * 16), (self.scales, (k + 31) // 32)):
+            if t.dtype != torch.uint8 or t.device != device or tuple(t.shape) != (self.shape[0], w) or not t.is_contiguous():
+                raise DiffGraphHipError(f"{name}: its codes and scales are not checkpoint8's, or on another device than {device}")
+        if self.shape[0] != n:
+            raise DiffGraphHipError(f"{name}: kept of {self.shape[0]} rows, the gradient has {n}")
+
+
+def checkpoint8(x: torch.Tensor, format: str = "int8") -> Checkpoint8:
+    """x [n, k] (float32 / bfloat16 / float16) in 8 bits: codes of `format` "int8" or "e4m3" and, per 32 columns of a row,
+    the smallest power of two that keeps the group's largest within them; each value to the nearest code (ties to even)."""
+    _rows(x, "x")
+    if format not in _FORMATS:
+        raise DiffGraphHipError(f"format: 'int8' or 'e4m3', got {format!r}")
+    n, k = x.shape
+    dev = x.device
+    with _lib.on_device(dev):
+        codes = torch.empty((n, (k + 15) // 16 * 16), dtype=torch.uint8, device=dev)
+        scales = torch.empty((n, (k + 31) // 32), dtype=torch.uint8, device=dev)
+        rc = _lib.load().dg_checkpoint8(x.data_ptr(), x.stride(0), n, k, _ELEMENT[x.dtype], _FORMATS[format], codes.data_ptr(),
+                                        scales.data_ptr(), _lib.stream_ptr(dev))
+        _lib.check(rc, "dg_checkpoint8")
+    return Checkpoint8(codes, scales, (n, k), format)
+
+
+def checkpoint8_backward(d_y: torch.Tensor, x: Checkpoint8, y: Optional[Checkpoint8] = None):
+    """(d_z [n, m], d_w [m, k], d_b [m]), of d_y's type, of a dense layer z = x . w^T + b from the gradient d_y [n, m] and
+    what was kept of its input x [n, k]: d_w = d_z^T . x, d_b = column sums of d_z, where d_z is d_y (returned as it is), or,
+    with what was kept of y = tanh(z), d_y (1 - y y).  Sums in fp32 in a fixed order."""
+    _rows(d_y, "d_y")
+    n, m = d_y.shape
+    dev = d_y.device
+    Checkpoint8.check(x, "x", n, dev)
+    k = x.shape[1]
+    if y is not None:
+        Checkpoint8.check(y, "y", n, dev)
+        if y.shape[1] != m or y.format != x.format:
+            raise DiffGraphHipError(f"y: expected {m} columns in the format of x ({x.format})")
+    lib = _lib.load()
+    with _lib.on_device(dev):
+        ws_bytes = int(lib.dg_checkpoint8_backward_workspace(n, k, m))
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        d_z = d_y if y is None else torch.empty((n, m), dtype=d_y.dtype, device=dev)
+        d_w = torch.empty((m, k), dtype=d_y.dtype, device=dev)
+        d_b = torch.empty(m, dtype=d_y.dtype, device=dev)
+        rc = lib.dg_checkpoint8_backward(d_y.data_ptr(), d_y.stride(0), n, m, k, _ELEMENT[d_y.dtype], _FORMATS[x.format],
+                                         x.codes.data_ptr(), x.scales.data_ptr(), None if y is None else y.codes.data_ptr(),
+                                         None if y is None else y.scales.data_ptr(), d_z.data_ptr(), d_w.data_ptr(), d_b.data_ptr(),
+                                         ws.data_ptr(), ws_bytes, _lib.stream_ptr(dev))
+        _lib.check(rc, "dg_checkpoint8_backward")
+    return d_z, d_w, d_b

@@ -14,7 +14,7 @@ for s in ${VARIANT_SOURCES:-spmm graph}; do
   /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Wall -Wno-unused-function -Xclang -target-feature -Xclang -packed-fp32-ops "$@" -c $C/$s.hip -o scratch/${s}_$tag.o
 done
 objs=""
-for s in graph spmm fused diffusion wgrad losshead eval sampling spgemm optim linear comm embedding scores; do
+for s in graph spmm fused diffusion wgrad losshead eval sampling spgemm optim linear comm embedding scores checkpoint8; do
   if [ -f scratch/${s}_$tag.o ]; then objs="$objs scratch/${s}_$tag.o"; else objs="$objs $C/$s.o"; fi
 done
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o scratch/libdg_$tag.so $objs -ldl
