@@ -50,12 +50,49 @@ class _LinearFn(torch.autograd.Function):
         return d_x, d_w, d_b
 
 
+class _Dense8Fn(torch.autograd.Function):
+    """nn.Linear, with tanh behind it or not, that keeps its input and its tanh output in 8 bits for the backward pass
+    (ops.checkpoint8): a quarter of the bytes, the same forward values.  The codes of an output are handed on, so that the
+    layer behind it keeps nothing of its own.  The gradient of the input is exact; d_w and tanh' are formed from the codes."""
+
+    @staticmethod
+    def forward(ctx, x, codes, scales, w, b, fmt, tanh):
+        x, w = x.contiguous(), w.contiguous()
+        xk = ops.checkpoint8(x, fmt) if codes is None else ops.Checkpoint8(codes, scales, tuple(x.shape), fmt)
+        y = ops.linear_fwd(x, w, b)
+        yk = None
+        if tanh:
+            y = torch.tanh(y)
+            yk = ops.checkpoint8(y, fmt)
+        ctx.save_for_backward(w, xk.codes, xk.scales, *((yk.codes, yk.scales) if tanh else ()))
+        ctx.aux = (fmt, xk.shape, tuple(y.shape))
+        if not tanh:
+            return y, None, None
+        ctx.mark_non_differentiable(yk.codes, yk.scales)
+        return y, yk.codes, yk.scales
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, _codes, _scales):
+        w, xc, xs, *y = ctx.saved_tensors
+        fmt, x_shape, y_shape = ctx.aux
+        yk = ops.Checkpoint8(*y, y_shape, fmt) if y else None
+        d_z, d_w, d_b = ops.checkpoint8_backward(dy.contiguous(), ops.Checkpoint8(xc, xs, x_shape, fmt), yk)
+        d_x = ops.linear_fwd(d_z, w.t().contiguous(), None) if ctx.needs_input_grad[0] else None
+        return d_x, None, None, d_w, d_b, None, None
+
+
 class Denoise(nn.Module):
     """Denoise(in_dims, out_dims, emb_size, norm, dropout) -- Model.py:176-234.  `fused`: the layer shapes the fused
-    kernels are built for (in_dims = out_dims = [64, 64], emb_size 8); other shapes run layer by layer."""
+    kernels are built for (in_dims = out_dims = [64, 64], emb_size 8); other shapes run layer by layer.  act_ckpt
+    ("int8" / "e4m3"): the layer-by-layer form keeps its activations for the backward pass in 8 bits (the fused kernels
+    keep none and take no notice)."""
 
-    def __init__(self, in_dims, out_dims, emb_size, norm=False, dropout=0.5):
+    def __init__(self, in_dims, out_dims, emb_size, norm=False, dropout=0.5, act_ckpt=None):
         super().__init__()
+        if act_ckpt not in (None, "int8", "e4m3"):
+            raise ValueError(f"act_ckpt: None, 'int8' or 'e4m3', got {act_ckpt!r}")
+        self.act_ckpt = act_ckpt
         in_dims, out_dims = list(in_dims), list(out_dims)
         if len(in_dims) < 2 or len(out_dims) < 2 or in_dims[0] < 1 or out_dims[-1] != in_dims[0] or emb_size < 1:
             raise NotImplementedError(f"a denoiser takes and returns rows of one width (latdim), got in_dims {in_dims}, "
@@ -134,6 +171,13 @@ class Denoise(nn.Module):
             else:
                 x = self.drop(x)
         h = torch.cat([x, emb], dim=-1)
+        if self.act_ckpt is not None and torch.is_grad_enabled():
+            codes = scales = None
+            dense = [(layer, True) for layer in self.in_layers]
+            dense += [(layer, i != len(self.out_layers) - 1) for i, layer in enumerate(self.out_layers)]
+            for layer, tanh in dense:
+                h, codes, scales = _Dense8Fn.apply(h, codes, scales, layer.weight, layer.bias, self.act_ckpt, tanh)
+            return h if wide == self.width else torch.nn.functional.pad(h, (0, wide - self.width))
         for layer in self.in_layers:
             h = torch.tanh(_LinearFn.apply(h, layer.weight, layer.bias))
         for i, layer in enumerate(self.out_layers):

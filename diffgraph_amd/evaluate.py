@@ -13,7 +13,7 @@ from typing import Dict, List
 import numpy as np
 import torch
 
-from . import _lib
+from . import _lib, ops
 from ._lib import DG_D, DiffGraphHipError
 
 
@@ -87,6 +87,50 @@ def all_rank_topk(usrEmbeds: torch.Tensor, itmEmbeds: torch.Tensor, users: torch
                           data.trn_rowptr.data_ptr(), data.trn_col.data_ptr(), int(topk), DG_D, ws.data_ptr(), ws_bytes,
                           top_idx.data_ptr(), top_val.data_ptr(), _lib.stream_ptr(dev))
     _lib.check(rc, "dg_eval_topk")
+    return top_val, top_idx
+
+
+def recommend(usrEmbeds: torch.Tensor, itmEmbeds: torch.Tensor, users: torch.Tensor, data: AllRankTestData, topk: int = 20, *,
+              exclude: bool = True, repetition=None, frequency=None, presence=None, bias=None, allowed=None, allowed_rows=None,
+              batch: int = 1024):
+    """The topk items for int64 `users`, one or many, with what a service asks for beside all_rank_topk's mask: (values,
+    item ids int32), [len(users), topk], from t.mm(usrEmbeds[users], itmEmbeds.T) after ops.adjust_scores over the users'
+    training items as their history.  exclude (default): those items are out (-inf); otherwise repetition / frequency /
+    presence penalise them (a number, or float32 with one value per entry of `users`).  bias float32 [items] is added;
+    allowed / allowed_rows: int32 bit masks of the items that stay, per entry of `users`, as ops.adjust_scores takes them.
+    Tables of any width in float32, bfloat16 or float16; `batch` users at a time.  An item that is out has value -inf: it
+    comes back only where fewer than topk items are left.  A user outside the table gets NaN values."""
+    n, n_item = users.numel(), data.n_item
+    if usrEmbeds.dim() != 2 or itmEmbeds.dim() != 2 or usrEmbeds.shape[0] != data.n_user or itmEmbeds.shape[0] != n_item:
+        raise DiffGraphHipError("embedding tables do not match the interaction matrices")
+    if usrEmbeds.dtype != itmEmbeds.dtype or usrEmbeds.shape[1] != itmEmbeds.shape[1]:
+        raise DiffGraphHipError("embedding tables: expected one type and width")
+    if users.dtype != torch.int64 or users.dim() != 1 or not users.is_cuda:
+        raise DiffGraphHipError("users: expected a 1-D int64 GPU tensor")
+    if not 0 < topk <= n_item:
+        raise DiffGraphHipError(f"topk must lie in [1,{n_item}]; got {topk}")
+    if batch < 1:
+        raise DiffGraphHipError(f"batch must be positive, got {batch}")
+    if allowed is not None and allowed.dim() == 2 and allowed_rows is None and allowed.shape[0] not in (1, n):
+        raise DiffGraphHipError(f"allowed: {allowed.shape[0]} masks for {n} users: allowed_rows says which")
+    for nm, v in (("repetition", repetition), ("frequency", frequency), ("presence", presence), ("allowed_rows", allowed_rows)):
+        if isinstance(v, torch.Tensor) and v.shape != (n,):
+            raise DiffGraphHipError(f"{nm}: expected one value for each of {n} users")
+    if bias is not None and bias.dim() != 1:
+        raise DiffGraphHipError(f"bias: expected shape [{n_item}]")
+    usrEmbeds, itmEmbeds = usrEmbeds.detach(), itmEmbeds.detach()
+    top_val = torch.empty((n, topk), dtype=usrEmbeds.dtype, device=usrEmbeds.device)
+    top_idx = torch.empty((n, topk), dtype=torch.int32, device=usrEmbeds.device)
+    for b in range(0, n, batch):
+        part = slice(b, min(b + batch, n))
+        of = lambda v: v[part] if isinstance(v, torch.Tensor) else v  # noqa: E731
+        masks = allowed[part] if allowed is not None and allowed.dim() == 2 and allowed_rows is None and allowed.shape[0] == n else allowed
+        u = users[part]
+        scores = torch.mm(ops.embedding_lookup(usrEmbeds, u), itmEmbeds.t())
+        ops.adjust_scores(scores, history=(data.trn_rowptr, data.trn_col), rows=u, repetition=of(repetition), frequency=of(frequency),
+                          presence=of(presence), bias=bias, allowed=masks, allowed_rows=of(allowed_rows), exclude=exclude, out=scores)
+        v, i = torch.topk(scores, topk)
+        top_val[part], top_idx[part] = v, i.to(torch.int32)
     return top_val, top_idx
 
 

@@ -163,7 +163,8 @@ class HGDM(nn.Module):
         self.n_hid = args.latdim
         out_dims = eval(args.dims) + [args.latdim]
         in_dims = out_dims[::-1]
-        self.user_denoise_model = Denoise(in_dims, out_dims, args.d_emb_size, norm=args.norm).to(device)
+        act_ckpt = getattr(args, "act_ckpt", None)     # "int8" / "e4m3": a layer-by-layer denoiser keeps its activations in 8 bits
+        self.user_denoise_model = Denoise(in_dims, out_dims, args.d_emb_size, norm=args.norm, act_ckpt=act_ckpt).to(device)
         # (a denoiser outside the fused kernels' shape -- another --dims list or --d_emb_size -- runs layer by layer:
         # GaussianDiffusion.training_losses_rows and p_sample take either kind)
         self.diffusion_model = GaussianDiffusion(args.noise_scale, args.noise_min, args.noise_max, args.steps)

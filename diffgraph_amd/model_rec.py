@@ -250,8 +250,9 @@ class HGDM(nn.Module):
         self.diffusion_process = GaussianDiffusion(args.noise_scale, args.noise_min, args.noise_max, args.steps)
         out_dims = eval(args.dims) + [args.latdim]
         in_dims = out_dims[::-1]
-        self.usr_denoiser = Denoise(in_dims, out_dims, args.d_emb_size, norm=args.norm).to(device)
-        self.item_denoiser = Denoise(in_dims, out_dims, args.d_emb_size, norm=args.norm).to(device)
+        act_ckpt = getattr(args, "act_ckpt", None)     # "int8" / "e4m3": a layer-by-layer denoiser keeps its activations in 8 bits
+        self.usr_denoiser = Denoise(in_dims, out_dims, args.d_emb_size, norm=args.norm, act_ckpt=act_ckpt).to(device)
+        self.item_denoiser = Denoise(in_dims, out_dims, args.d_emb_size, norm=args.norm, act_ckpt=act_ckpt).to(device)
         # {seed, draws made, dropout key, 0} of the timesteps / noise / dropout masks drawn on the device; part of the
         # state_dict, so that a resumed run goes on with the draws that follow instead of repeating the first ones
         self.register_buffer("draw_state", ops.new_draw_state(device), persistent=True)

@@ -3,8 +3,9 @@
 The propagation is column-separable up to the row normalisation: y = LeakyReLU(A_hat x) holds column block by column
 block, so every 64-column block of a table goes through the same HIP propagation kernel (dg_spmm_norm_act_fwd, and its
 transposed form in the backward pass), and what couples the blocks -- F.normalize over the whole row, the layer sums,
-the loss head's dot products, the evaluation scores -- is formed by torch device ops under autograd, written as the
-reference writes them (Model.py:53-111).  The denoisers run layer by layer in the HIP dense-layer kernels
+the loss head's dot products, the evaluation's products -- is formed by torch device ops under autograd, written as the
+reference writes them (Model.py:53-111).  The batch's rows are looked up, and their gradient summed by token, by the HIP
+embedding kernels (layers.embedding); the training items leave the evaluation scores in one pass (ops.adjust_scores).  The denoisers run layer by layer in the HIP dense-layer kernels
 (diffusion.Denoise.forward_layers).  Correct for every width; tuned for none: the fused kernels are built for 64.
 """
 from __future__ import annotations
@@ -16,6 +17,7 @@ import torch.nn.functional as F
 
 from . import ops
 from ._lib import DG_D
+from .layers import embedding
 
 
 class _SpmmFn(torch.autograd.Function):
@@ -63,10 +65,10 @@ def cal_loss(model, ancs, poss, negs, ts_u=None, noise_u=None, ts_i=None, noise_
                         float(model.act.negative_slope))
     rl_u, out_u = dp.training_losses_rows(model.usr_denoiser, ui[:nu], het[:nu], ts_u, noise_u, keep_u)
     rl_i, out_i = dp.training_losses_rows(model.item_denoiser, ui[nu:], het[nu:], ts_i, noise_i, keep_i)
-    ancs, poss, negs = ancs.long(), poss.long(), negs.long()
+    ancs, poss, negs = (v.long().to(ui.device) for v in (ancs, poss, negs))
     diff = rl_u[ancs].mean() + rl_i[poss].mean()
     usr, itm = ui[:nu] + out_u, ui[nu:] + out_i
-    a, p, n = usr[ancs], itm[poss], itm[negs]
+    a, p, n = embedding(usr, ancs), embedding(itm, poss), embedding(itm, negs)
     score = (a * p).sum(-1) - (a * n).sum(-1)                                       # pairPredict (Utils/Utils.py:4-8)
     bpr = -score.sigmoid().log().sum() / args.batch
     reg = ((torch.norm(a) ** 2 + torch.norm(p) ** 2 + torch.norm(n) ** 2) * args.reg) / args.batch
@@ -76,20 +78,15 @@ def cal_loss(model, ancs, poss, negs, ts_u=None, noise_u=None, ts_i=None, noise_
 def all_rank_topk(usr: torch.Tensor, itm: torch.Tensor, users: torch.Tensor, trn_rowptr: torch.Tensor, trn_col: torch.Tensor,
                   topk: int, batch: int = 1024):
     """t.topk(t.mm(usr[users], itm^T) * (1 - trnMask) - trnMask * 1e8, topk) (main.py:157-158) in batches of users,
-    the mask rows scattered from the training CSR.  Returns (values [len(users), topk], item ids int32)."""
+    the training items of a row replaced by -1e8 in one pass.  Returns (values [len(users), topk], item ids int32)."""
     n_item = itm.shape[0]
+    usr, itm, users = usr.detach(), itm.detach(), users.long().to(usr.device)
+    usr = usr if usr.stride(1) == 1 else usr.contiguous()
     vals, idx = [], []
-    deg = (trn_rowptr[1:] - trn_rowptr[:-1]).long()
     for b in range(0, users.numel(), batch):
         u = users[b: b + batch]
-        mask = torch.zeros((u.numel(), n_item), dtype=usr.dtype, device=usr.device)
-        cnt = deg[u]
-        rows = torch.repeat_interleave(torch.arange(u.numel(), device=usr.device), cnt)
-        if rows.numel():
-            first = trn_rowptr[u].long()
-            offs = torch.arange(rows.numel(), device=usr.device) - torch.repeat_interleave(torch.cumsum(cnt, 0) - cnt, cnt)
-            mask[rows, trn_col[torch.repeat_interleave(first, cnt) + offs].long()] = 1.0
-        preds = torch.mm(usr[u], itm.t()) * (1 - mask) - mask * 1e8
+        preds = torch.mm(ops.embedding_lookup(usr, u), itm.t())
+        ops.adjust_scores(preds, history=(trn_rowptr, trn_col), rows=u, exclude=True, fill=-1e8, out=preds)
         v, i = torch.topk(preds, min(topk, n_item))
         vals.append(v)
         idx.append(i.to(torch.int32))

@@ -1,0 +1,275 @@
+"""The operators in the framework's own paths, one after the other as they are used: denoisers that keep their
+activations in 8 bits (Denoise(act_ckpt=...), args.act_ckpt), the wide model's batch rows by embedding lookup, its
+evaluation and evaluate.recommend over adjusted scores."""
+import copy
+import math
+from types import SimpleNamespace
+
+import numpy as np
+import pytest
+import torch
+
+import diffgraph_amd as dg
+from diffgraph_amd import DiffGraphHipError, data as dgdata, evaluate as ev, ops
+from diffgraph_amd.model_rec import DEFAULT_ARGS
+from tests.helpers import GRAD_TOL, assert_close_to_max, assert_rows_close
+
+gpu = pytest.mark.gpu
+DEV = "cuda"
+
+
+def denoiser(fmt, latdim=96, dims=(128, 40), emb=10, seed=0):
+    torch.manual_seed(seed)
+    out = list(dims) + [latdim]
+    return dg.Denoise(out[::-1], out, emb, norm=True, act_ckpt=fmt).to(DEV)
+
+
+def dense_layers(dn):
+    return [(l, True) for l in dn.in_layers] + [(l, i != len(dn.out_layers) - 1) for i, l in enumerate(dn.out_layers)]
+
+
+@gpu
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("n", [1, 77, 1500])
+def test_denoiser_forward_is_unchanged_and_gradients_follow_the_kept_values(n, fmt):
+    dn, plain = denoiser(fmt), denoiser(None)
+    plain.load_state_dict(dn.state_dict())
+    x = torch.randn(n, 96, device=DEV, requires_grad=True)
+    t = torch.randint(0, 200, (n,), device=DEV)
+    keep = torch.rand(n, 96, device=DEV) < 0.5
+    out = dn(x, t, True, keep)
+    assert torch.equal(out, plain(x.detach(), t, True, keep))                   # the same forward values
+    with torch.no_grad():
+        assert torch.equal(out, dn(x, t, True, keep))
+    d_out = torch.randn_like(out)
+    out.backward(d_out)
+    # the backward pass in 64 bits, from the values that the codes of the very same activations stand for
+    acts = []
+    with torch.no_grad():
+        e = torch.arange(5, device=DEV, dtype=torch.float32)
+        f = t[:, None].float() * torch.exp(-math.log(10000) * e / 5)[None]
+        emb = ops.linear_fwd(torch.cat([torch.cos(f), torch.sin(f)], 1).contiguous(), dn.emb_layer.weight, dn.emb_layer.bias)
+        h = torch.cat([torch.nn.functional.normalize(x) * (keep.float() * 2.0), emb], 1)
+        for layer, tanh in dense_layers(dn):
+            kept = ops.checkpoint8(h, fmt).values().double()
+            h = ops.linear_fwd(h.contiguous(), layer.weight, layer.bias)
+            h = torch.tanh(h) if tanh else h
+            acts.append((kept, ops.checkpoint8(h, fmt).values().double() if tanh else None))
+        assert torch.equal(h, out)
+    d = d_out.double()
+    for (layer, tanh), (xv, yv) in reversed(list(zip(dense_layers(dn), acts))):
+        d = d * (1 - yv * yv) if tanh else d
+        assert_close_to_max(layer.weight.grad, d.t() @ xv, GRAD_TOL, "d weight")
+        assert_close_to_max(layer.bias.grad, d.sum(0), GRAD_TOL, "d bias")
+        d = d @ layer.weight.detach().double()
+    xd = x.detach().double().requires_grad_()
+    (torch.nn.functional.normalize(xd) * (keep.double() * 2.0)).backward(d[:, :96])
+    # (through normalize, whose backward takes g's part along the row away: what is left may be a tenth of g)
+    assert_rows_close(x.grad, xd.grad, rtol=1e-4, what="d x")
+    # and they stay within what the rounding of the codes explains: the last layer's weight, whose d_z is the same
+    x2 = x.detach().requires_grad_()
+    plain(x2, t, True, keep).backward(d_out)
+    last, ref = dn.out_layers[-1].weight.grad.double(), plain.out_layers[-1].weight.grad.double()
+    half = 2.0 ** -7 if fmt == "int8" else 2.0 ** -4                  # of |h| <= 1: half a scale of at most 2^-6; half a step
+    bound = half * d_out.double().abs().sum(0)[:, None] + GRAD_TOL * ref.abs().max()
+    assert bool(((last - ref).abs() <= bound).all())
+
+
+@gpu
+def test_kept_bytes():
+    """What autograd holds between the passes, apart from the weights: a quarter of the fp32 activations and a little."""
+    n, held = 4096, {}
+    for fmt in (None, "int8"):
+        dn = denoiser(fmt, dims=(256, 128))
+        weights = {p.data_ptr() for p in dn.parameters()}
+        seen = {}
+
+        def pack(v):
+            if v.data_ptr() not in weights:
+                seen[v.data_ptr()] = v.numel() * v.element_size()
+            return v
+        x, t = torch.randn(n, 96, device=DEV), torch.randint(0, 200, (n,), device=DEV)
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda v: v):
+            out = dn(x, t, False)
+        held[fmt] = sum(seen.values())
+        del out
+    # per row: 106 + 128 + 256 + 128 inner columns... each a byte and its scale's share, the time embedding's 10 floats beside them
+    cols = 96 + 10 + 128 + 256 + 128
+    assert held["int8"] <= n * (cols * 1.2 + 2 * 10 * 4 + 64) < 0.45 * held[None]
+
+
+@gpu
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_backward_against_differences(fmt):
+    """One row, its bias chosen so that tanh(z) is a code's value: d_w is then the gradient of sum c tanh(x^ w^T + b)."""
+    torch.manual_seed(4)
+    m, k = 9, 40
+    x = ops.checkpoint8(torch.randn(1, k, device=DEV), fmt)
+    y = ops.checkpoint8(torch.tanh(torch.randn(1, m, device=DEV)) * 0.9, fmt)
+    xv, yv = x.values().double(), y.values().double()
+    c = torch.randn(1, m, device=DEV)
+    _, d_w, d_b = ops.checkpoint8_backward(c, x, y)
+    w = torch.randn(m, k, dtype=torch.float64, device=DEV)
+    b = torch.atanh(yv) - xv @ w.t()
+    loss = lambda w, b: (c.double() * torch.tanh(xv @ w.t() + b)).sum()  # noqa: E731
+    h = 1e-5
+    for o, i in ((0, 0), (8, 39), (4, 31), (5, 32)):
+        e = torch.zeros_like(w)
+        e[o, i] = h
+        diff = float(loss(w + e, b) - loss(w - e, b)) / (2 * h)
+        # central difference: (h x)^2 / 6 of the third derivative (at most 2) and 64-bit rounding / h; the kernel: three roundings
+        tol = abs(float(c[0, o])) * (abs(float(xv[0, i])) ** 3 * h * h + 1e-10) + 4 * 2.0 ** -24 * abs(diff) + 1e-10
+        assert abs(float(d_w[o, i]) - diff) <= tol
+        e = torch.zeros_like(b)
+        e[0, o] = h
+        diff = float(loss(w, b + e) - loss(w, b - e)) / (2 * h)
+        assert abs(float(d_b[o]) - diff) <= abs(float(c[0, o])) * (h * h + 1e-10) + 4 * 2.0 ** -24 * abs(diff) + 1e-10
+
+
+def test_denoiser_refuses_another_format():
+    with pytest.raises(ValueError, match="act_ckpt"):
+        dg.Denoise([96, 40], [40, 96], 8, act_ckpt="int4")
+
+
+@gpu
+@pytest.mark.parametrize("use_graph", [False, True])
+@pytest.mark.parametrize("fmt,latdim", [("int8", 64), ("e4m3", 128)])
+def test_coach_epochs_with_kept_activations_then_recommendations(fmt, latdim, use_graph):
+    """A run of all three together: training steps whose denoisers keep 8 bits (at latdim 128 the batch rows by lookup and
+    gradient by token), eagerly and recorded; evaluation; recommendations out of the trained tables."""
+    from diffgraph_amd.train import Coach
+    from tests.test_gpu_train import _handler
+    args = copy.copy(DEFAULT_ARGS)
+    args.batch, args.dims, args.d_emb_size, args.epoch, args.latdim, args.act_ckpt = 64, "[128, 32]", 10, 2, latdim, fmt
+    torch.manual_seed(5)
+    handler = _handler()
+    c = Coach(handler, args, device=DEV, use_graph=use_graph, seed=3)
+    lines = []
+    res = c.run(log=lines.append)
+    assert c.model.usr_denoiser.act_ckpt == fmt and not c.model.usr_denoiser.fused
+    assert len(lines) == 4 and all("nan" not in ln.lower() for ln in lines), lines
+    assert 0.0 <= res["Recall"] <= 1.0
+    with torch.no_grad():
+        pu, pi = c.model.predict()
+    data = handler.tst_data
+    val, idx = ev.recommend(pu, pi, data.test_users_dev, data, 5)
+    v2, i2 = ev.all_rank_topk(pu, pi, data.test_users_dev, data, 5)
+    kept = torch.isfinite(val)
+    np.testing.assert_allclose(val[kept].cpu().numpy(), v2[kept].cpu().numpy(), rtol=2e-5, atol=2e-5 * float(v2[kept].abs().max()))
+    assert i2.shape == idx.shape
+
+
+@gpu
+def test_recorded_and_eager_steps_agree_with_kept_activations():
+    """The same draws, the same steps: a recorded training step with 8-bit activations gives the eager step's bits."""
+    from diffgraph_amd.train import Coach
+    from tests.test_gpu_train import _handler
+    got = []
+    for use_graph in (False, True):
+        args = copy.copy(DEFAULT_ARGS)
+        args.batch, args.dims, args.epoch, args.latdim, args.act_ckpt = 64, "[48]", 1, 128, "int8"
+        torch.manual_seed(6)
+        handler = _handler()
+        c = Coach(handler, args, device=DEV, use_graph=use_graph, seed=3)
+        c.prepareModel()
+        # (the warm-up steps before a recording take draws beyond the step's own and give them back: a few more than steps)
+        n, steps = c.model.n_user + c.model.n_item, c._n_batches + 4
+        g = torch.Generator().manual_seed(9)
+        c.set_draws(torch.randint(0, 200, (steps, n), generator=g), torch.randn(steps, n, 128, generator=g),
+                    (torch.rand(steps, n, 128, generator=g) < 0.5).to(torch.uint8))
+        c.trainEpoch()
+        got.append([p.detach().clone() for p in c.model.parameters()])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+# ---- wide model, evaluation, recommendations ------------------------------------------------------------------------
+def interactions(nu, ni, seed=3):
+    import scipy.sparse as sp
+    trn_u, trn_i = dgdata.synth_interactions(nu, ni, nu * 20, seed)
+    rng = np.random.default_rng(5)
+    coo = lambda u, i: sp.coo_matrix((np.ones(len(u), np.float32), (u, i)), shape=(nu, ni))  # noqa: E731
+    data = ev.AllRankTestData(coo(np.arange(nu, dtype=np.int32), rng.integers(0, ni, nu).astype(np.int32)), coo(trn_u, trn_i))
+    had = torch.zeros(nu, ni, dtype=torch.bool)
+    had[torch.from_numpy(trn_u).long(), torch.from_numpy(trn_i).long()] = True
+    return data, had
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("width", [64, 100])
+def test_recommend(width, dtype):
+    nu, ni, k = 70, 900, 20
+    data, had = interactions(nu, ni)
+    g = torch.Generator().manual_seed(1)
+    usr, itm = torch.randn(nu, width, generator=g).to(dtype).to(DEV), torch.randn(ni, width, generator=g).to(dtype).to(DEV)
+    users = torch.tensor([3, 69, 3, 0, 41], device=DEV)
+    scores = torch.mm(usr[users], itm.t())                        # the operators' part starts here
+    rep = torch.tensor([1.0, 1.5, 2.0, 1.2, 0.9], device=DEV)
+    bias = torch.randn(ni, generator=g).to(DEV)
+    words = torch.randint(-2 ** 31, 2 ** 31, (3, (ni + 31) // 32), generator=g).to(torch.int32).to(DEV)
+    which = torch.tensor([0, -1, 2, 1, 1], dtype=torch.int32, device=DEV)
+    stays = ((words.cpu().long()[:, torch.arange(ni) // 32] >> (torch.arange(ni) % 32)) & 1).bool()
+    for exclude, batch in ((True, 1024), (False, 2)):
+        val, idx = ev.recommend(usr, itm, users, data, k, exclude=exclude, repetition=rep, presence=0.1, bias=bias, allowed=words,
+                                allowed_rows=which, batch=batch)
+        assert val.dtype == dtype and idx.dtype == torch.int32 and val.shape == idx.shape == (5, k)
+        s, h = scores.cpu().double(), had[users.cpu()]
+        r = rep.cpu().double()[:, None]
+        s = torch.where(h, torch.where(s > 0, s / r, s * r) - 0.1, s) + bias.cpu().double()
+        out = ~(stays[which.cpu().long().clamp(min=0)] | (which.cpu() < 0)[:, None])
+        s[out | h if exclude else out] = -math.inf
+        want = s.topk(k).values
+        # each score: four fp32 roundings of values below size, one to the type; a product of another shape may differ in
+        # its last bit itself (2 eps of its value)
+        size = s.masked_fill(torch.isinf(s), 0).abs().max() + 4
+        tol = 8 * 2.0 ** -24 * size + 3 * torch.finfo(dtype).eps * size
+        assert torch.equal(torch.isinf(val).cpu(), torch.isinf(want))
+        fin = torch.isfinite(want)
+        assert bool(((val.cpu().double() - want).abs()[fin] <= tol).all())
+        at = s.gather(1, idx.cpu().long())
+        assert bool(((at - val.cpu().double()).abs()[fin] <= tol).all())
+    one = ev.recommend(usr, itm, users[:1], data, 1)
+    assert one[0].shape == (1, 1) and not bool(had[3, int(one[1])])
+    assert ev.recommend(usr, itm, users[:0], data, 3)[0].shape == (0, 3)
+    odd = ev.recommend(usr, itm, torch.tensor([nu, 2], device=DEV), data, 3)
+    assert bool(odd[0][0].isnan().all()) and bool(odd[0][1].isfinite().all())
+
+
+@gpu
+def test_recommend_refusals():
+    data, _ = interactions(30, 50)
+    usr, itm, users = torch.zeros(30, 8, device=DEV), torch.zeros(50, 8, device=DEV), torch.tensor([1, 2], device=DEV)
+    for args, kw, what in (((usr[:29], itm, users), {}, "match"), ((usr, itm.half(), users), {}, "one type"), ((usr, itm, users.int()), {}, "users"),
+                           ((usr, itm, users), dict(topk=0), "topk"), ((usr, itm, users), dict(topk=51), "topk"), ((usr, itm, users), dict(batch=0), "batch"),
+                           ((usr, itm, users), dict(repetition=torch.ones(3, device=DEV)), "repetition"),
+                           ((usr, itm, users), dict(bias=torch.ones(2, 50, device=DEV)), "bias"),
+                           ((usr, itm, users), dict(allowed=torch.zeros(5, 2, dtype=torch.int32, device=DEV)), "allowed")):
+        with pytest.raises(DiffGraphHipError, match=what):
+            ev.recommend(args[0], args[1], args[2], data, **kw)
+
+
+@gpu
+def test_wide_loss_with_rows_named_many_times():
+    """wide.cal_loss: the gradient of a batch that names rows many times is the sum over the batch."""
+    from diffgraph_amd import wide
+    wl = dgdata.rec_workload("tiny")
+    nu, ni = wl.n_user, wl.n_item
+    graphs = [dg.CSRGraph.from_bipartite(u, i, nu, ni) for (u, i) in [wl.target] + wl.behaviours]
+    handler = SimpleNamespace(userNum=nu, itemNum=ni, target_adj=graphs[0], behavior_mats=graphs[1:])
+    args = SimpleNamespace(**{**vars(DEFAULT_ARGS), "latdim": 80, "batch": 300, "act_ckpt": "int8"})
+    torch.manual_seed(1)
+    m = dg.rec.HGDM(handler, args).eval()
+    n = 300
+    ids = [torch.randint(0, hi, (n,), device=DEV) for hi in (3, 2, ni)]
+    draws = (torch.randint(0, 200, (nu,), device=DEV), torch.randn(nu, 80, device=DEV), torch.randint(0, 200, (ni,), device=DEV),
+             torch.randn(ni, 80, device=DEV))
+    grads = []
+    for lookup in (wide.embedding, lambda table, i: table[i]):         # the kernels, and torch's own indexing
+        old, wide.embedding = wide.embedding, lookup
+        try:
+            m.zero_grad()
+            wide.cal_loss(m, *ids, *draws)[0].backward()
+        finally:
+            wide.embedding = old
+        grads.append(m.embedding_table.grad.clone())
+    assert_rows_close(grads[0], grads[1], rtol=1e-5, what="table gradient")
