@@ -251,11 +251,19 @@ def device_guard(device=None):
     return torch.cuda.device(device)
 
 
-def on_device(device):
-    """Context in which `device` (a tensor's) is the current GPU, so that a launch on its stream goes there."""
-    import contextlib
+def launch(device, fn, what: str, *args) -> None:
+    """fn(*args, stream) on `device` (a tensor's) and its current stream; raises on an error code.  Makes the device current
+    where it is not.  (torch's own lookups of the current device and stream, without the objects round them: the small
+    operators are bound by their host time.)"""
     import torch
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    at = device.index
+    if at == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(at))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(at))
+    if rc != 0:
+        check(rc, what)
 
 
 def stream_ptr(device=None) -> int:

@@ -25,48 +25,67 @@ __device__ __forceinline__ dg_bf16 dg_round<dg_bf16>(float v) {
   return {__builtin_bit_cast(uint16_t, (__bf16)v)};
 }
 
+template <int BYTES, int ALIGN>
+struct dg_words {
+  typedef uint32_t type __attribute__((ext_vector_type(BYTES / 4), aligned(ALIGN)));
+};
+
+// VEC elements as they lie in memory.
 template <typename T, int VEC>
-struct alignas(sizeof(T) * VEC) dg_vec {
+struct dg_vec {
   T v[VEC];
 };
 
-template <int VEC, typename T>
-__device__ __forceinline__ void dg_load(const T *p, float (&f)[VEC]) {
-  const dg_vec<T, VEC> w = *reinterpret_cast<const dg_vec<T, VEC> *>(p);
+// (through a vector of words: element-wise stores of a struct end up as such)
+template <int VEC, int ALIGN, typename T>
+__device__ __forceinline__ dg_vec<T, VEC> dg_load_raw(const T *p) {
+  dg_vec<T, VEC> w;
+  if constexpr (VEC == 1) {
+    w.v[0] = *p;
+  } else {
+    typedef typename dg_words<sizeof(T) * VEC, ALIGN>::type words;
+    const words q = *reinterpret_cast<const words *>(p);
+    __builtin_memcpy(&w, &q, sizeof(w));
+  }
+  return w;
+}
+
+template <int VEC, int ALIGN, typename T>
+__device__ __forceinline__ void dg_store_raw(T *p, const dg_vec<T, VEC> &w) {
+  if constexpr (VEC == 1) {
+    *p = w.v[0];
+  } else {
+    typedef typename dg_words<sizeof(T) * VEC, ALIGN>::type words;
+    words q;
+    __builtin_memcpy(&q, &w, sizeof(w));
+    *reinterpret_cast<words *>(p) = q;
+  }
+}
+
+template <int VEC, int ALIGN, typename T>
+__device__ __forceinline__ void dg_load_at(const T *p, float (&f)[VEC]) {
+  const dg_vec<T, VEC> w = dg_load_raw<VEC, ALIGN>(p);
 #pragma unroll
   for (int e = 0; e < VEC; ++e) f[e] = dg_widen(w.v[e]);
 }
 
-template <int VEC, typename T>
-__device__ __forceinline__ void dg_store(T *p, const float (&f)[VEC]) {
+template <int VEC, int ALIGN, typename T>
+__device__ __forceinline__ void dg_store_at(T *p, const float (&f)[VEC]) {
   dg_vec<T, VEC> w;
 #pragma unroll
   for (int e = 0; e < VEC; ++e) w.v[e] = dg_round<T>(f[e]);
-  *reinterpret_cast<dg_vec<T, VEC> *>(p) = w;
+  dg_store_raw<VEC, ALIGN>(p, w);
 }
 
-// The same for rows that start anywhere: the hardware takes vector accesses at any address of an element (a few more
-// cache lines touched), so only the ends of a row go element by element.
-template <int BYTES>
-struct dg_words {
-  typedef uint32_t type __attribute__((ext_vector_type(BYTES / 4), aligned(2)));
-};
-
+// Rows that start on 16 bytes.
 template <int VEC, typename T>
-__device__ __forceinline__ void dg_load_unaligned(const T *p, float (&f)[VEC]) {
-  const typename dg_words<sizeof(T) * VEC>::type q = *reinterpret_cast<const typename dg_words<sizeof(T) * VEC>::type *>(p);
-  T w[VEC];
-  __builtin_memcpy(w, &q, sizeof(w));
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) f[e] = dg_widen(w[e]);
-}
-
+__device__ __forceinline__ void dg_load(const T *p, float (&f)[VEC]) { dg_load_at<VEC, 16>(p, f); }
 template <int VEC, typename T>
-__device__ __forceinline__ void dg_store_unaligned(T *p, const float (&f)[VEC]) {
-  T w[VEC];
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) w[e] = dg_round<T>(f[e]);
-  typename dg_words<sizeof(T) * VEC>::type q;
-  __builtin_memcpy(&q, w, sizeof(w));
-  *reinterpret_cast<typename dg_words<sizeof(T) * VEC>::type *>(p) = q;
-}
+__device__ __forceinline__ void dg_store(T *p, const float (&f)[VEC]) { dg_store_at<VEC, 16>(p, f); }
+
+// Rows that start anywhere: the hardware takes vector accesses at any address of an element (a few more cache lines
+// touched), so only the ends of a row go element by element.
+template <int VEC, typename T>
+__device__ __forceinline__ void dg_load_unaligned(const T *p, float (&f)[VEC]) { dg_load_at<VEC, 2>(p, f); }
+template <int VEC, typename T>
+__device__ __forceinline__ void dg_store_unaligned(T *p, const float (&f)[VEC]) { dg_store_at<VEC, 2>(p, f); }

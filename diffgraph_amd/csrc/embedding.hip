@@ -42,6 +42,7 @@ __global__ __launch_bounds__(256) void embedding_lookup_kernel(const T *__restri
 // Passes over at most kMaxDigit bits, low digit first; ids that take no gradient (outside the table, the padding id) get
 // the key n_rows, behind all others.  A pass: digit counts per block, per-digit scans over the blocks, stable scatter.
 constexpr int kMaxDigit = 10, kWaves = 4;
+constexpr int kSelfScan = 64;     // up to so many blocks a scatter adds their counts up itself (one launch less)
 
 struct key_source {
   const void *ids;      // first pass: the caller's ids
@@ -51,37 +52,57 @@ struct key_source {
   const uint32_t *keys, *pos;   // later passes
 };
 
-__device__ __forceinline__ void load_key(const key_source &s, int64_t i, uint32_t &key, uint32_t &pos) {
+// N entries, `step` apart, all on their way at once (an entry behind the list: some other one, to be left aside).
+template <int N>
+__device__ __forceinline__ void load_keys(const key_source &s, int64_t first, int step, int64_t n, uint32_t (&key)[N], uint32_t (&pos)[N]) {
   if (s.keys) {
-    key = s.keys[i];
-    pos = s.pos[i];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const int64_t i = min(first + e * step, n - 1);
+      key[e] = s.keys[i];
+      pos[e] = s.pos[i];
+    }
     return;
   }
-  const int64_t id = s.ids64 ? ((const int64_t *)s.ids)[i] : (int64_t)((const int32_t *)s.ids)[i];
-  key = ((uint64_t)id >= (uint64_t)s.n_rows || id == s.padding) ? s.n_rows : (uint32_t)id;
-  pos = (uint32_t)i;
+  int64_t id[N];
+  if (s.ids64) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) id[e] = ((const int64_t *)s.ids)[min(first + e * step, n - 1)];
+  } else {
+    int32_t low[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) low[e] = ((const int32_t *)s.ids)[min(first + e * step, n - 1)];
+#pragma unroll
+    for (int e = 0; e < N; ++e) id[e] = low[e];
+  }
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    key[e] = ((uint64_t)id[e] >= (uint64_t)s.n_rows || id[e] == s.padding) ? s.n_rows : (uint32_t)id[e];
+    pos[e] = (uint32_t)(first + e * step);
+  }
 }
 
-// counts[digit][block]
+// counts[digit][block], or [block][digit] where the scatter adds the blocks up itself
 template <int IPT>
-__global__ __launch_bounds__(256) void radix_count_kernel(key_source s, int64_t n, int shift, int bits, int n_blocks,
-                                                          uint32_t *__restrict__ counts) {
+__global__ __launch_bounds__(256) void radix_count_kernel(key_source s, int64_t n, int shift, int bits, int n_blocks, int by_block,
+                                                          uint32_t *__restrict__ counts, uint32_t *__restrict__ n_crossing) {
+  if (blockIdx.x == 0 && threadIdx.x == 0) *n_crossing = 0;
   __shared__ uint32_t hist[1 << kMaxDigit];
   const int bins = 1 << bits;
   for (int d = threadIdx.x; d < bins; d += 256) hist[d] = 0;
   __syncthreads();
   const int64_t base = (int64_t)blockIdx.x * (256 * IPT);
+  uint32_t key[IPT], pos[IPT];
+  load_keys<IPT>(s, base + threadIdx.x, 256, n, key, pos);
 #pragma unroll
-  for (int r = 0; r < IPT; ++r) {
-    const int64_t i = base + r * 256 + threadIdx.x;
-    if (i < n) {
-      uint32_t key, pos;
-      load_key(s, i, key, pos);
-      atomicAdd(&hist[(key >> shift) & (bins - 1)], 1u);   // (whole numbers: any order gives the same counts)
-    }
-  }
+  for (int r = 0; r < IPT; ++r)
+    if (base + r * 256 + threadIdx.x < n) atomicAdd(&hist[(key[r] >> shift) & (bins - 1)], 1u);   // (whole numbers: any order)
   __syncthreads();
-  for (int d = threadIdx.x; d < bins; d += 256) counts[(size_t)d * n_blocks + blockIdx.x] = hist[d];
+  if (by_block) {
+    for (int d = threadIdx.x; d < bins; d += 256) counts[(size_t)blockIdx.x * bins + d] = hist[d];
+  } else {
+    for (int d = threadIdx.x; d < bins; d += 256) counts[(size_t)d * n_blocks + blockIdx.x] = hist[d];
+  }
 }
 
 __device__ __forceinline__ uint32_t wave_inclusive(uint32_t v) {
@@ -123,6 +144,24 @@ __global__ __launch_bounds__(256) void radix_scan_kernel(uint32_t *__restrict__ 
   if (threadIdx.x == 0) totals[blockIdx.x] = carry;
 }
 
+template <int PER>
+__device__ __forceinline__ void sum_blocks(const uint32_t *__restrict__ counts, int bins, int n_blocks, uint32_t (&all)[4],
+                                           uint32_t (&before)[4]) {
+#pragma unroll 16
+  for (int b = 0; b < n_blocks; ++b) {
+    uint32_t c[PER];
+    const uint32_t *src = counts + (size_t)b * bins;       // (bins and the digit are multiples of PER)
+    if constexpr (PER == 1) c[0] = *src;
+    if constexpr (PER == 2) { const uint2 v = *reinterpret_cast<const uint2 *>(src); c[0] = v.x; c[1] = v.y; }
+    if constexpr (PER == 4) { const uint4 v = *reinterpret_cast<const uint4 *>(src); c[0] = v.x; c[1] = v.y; c[2] = v.z; c[3] = v.w; }
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+      all[q] += c[q];
+      before[q] += b < (int)blockIdx.x ? c[q] : 0;
+    }
+  }
+}
+
 template <int IPT>
 __global__ __launch_bounds__(256) void radix_scatter_kernel(key_source s, int64_t n, int shift, int bits, int n_blocks,
                                                             const uint32_t *__restrict__ counts, const uint32_t *__restrict__ totals,
@@ -134,24 +173,38 @@ __global__ __launch_bounds__(256) void radix_scatter_kernel(key_source s, int64_
   for (int d = threadIdx.x; d < bins; d += 256)
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) seen[w][d] = 0;
-  uint32_t carry = 0;
-  for (int d0 = 0; d0 < bins; d0 += 256) {
-    const int d = d0 + threadIdx.x;
-    uint32_t total;
-    const uint32_t ex = block_exclusive(d < bins ? totals[d] : 0, wave_sums, total);
-    if (d < bins) base[d] = carry + ex + counts[(size_t)d * n_blocks + blockIdx.x];
-    carry += total;
+  // a thread takes bins / 256 neighbouring digits: their entries, and those of the blocks before this one
+  const int per = max(1, bins >> 8), d0 = threadIdx.x * per;
+  uint32_t all[4] = {0, 0, 0, 0}, before[4] = {0, 0, 0, 0}, sum = 0, total;
+  if (d0 < bins) {
+    if (totals) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (q < per) {
+          all[q] = totals[d0 + q];
+          before[q] = counts[(size_t)(d0 + q) * n_blocks + blockIdx.x];
+        }
+    } else if (per == 1) {
+      sum_blocks<1>(counts + d0, bins, n_blocks, all, before);
+    } else if (per == 2) {
+      sum_blocks<2>(counts + d0, bins, n_blocks, all, before);
+    } else {
+      sum_blocks<4>(counts + d0, bins, n_blocks, all, before);
+    }
   }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) sum += all[q];
+  uint32_t at = block_exclusive(sum, wave_sums, total);
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    if (q < per && d0 < bins) {
+      base[d0 + q] = at + before[q];
+      at += all[q];
+    }
   __syncthreads();
   uint32_t key[IPT], pos[IPT], rank[IPT];
   const int64_t first = (int64_t)blockIdx.x * (256 * IPT) + wave * (64 * IPT);   // a wave's items are neighbours
-#pragma unroll
-  for (int r = 0; r < IPT; ++r) {
-    const int64_t i = first + r * 64 + lane;
-    key[r] = 0; pos[r] = 0;
-    if (i < n) load_key(s, i, key[r], pos[r]);
-  }
-  volatile uint32_t *mine = seen[wave];
+  load_keys<IPT>(s, first + lane, 64, n, key, pos);
 #pragma unroll
   for (int r = 0; r < IPT; ++r) {
     const bool in = first + r * 64 + lane < n;
@@ -162,11 +215,11 @@ __global__ __launch_bounds__(256) void radix_scatter_kernel(key_source s, int64_
       same &= (d >> b) & 1 ? set : ~set;
     }
     const uint32_t below = __popcll(same & ((1ull << lane) - 1));
-    const uint32_t before = in ? mine[d] : 0;
+    const uint32_t before = in ? seen[wave][d] : 0;
     rank[r] = before + below;
-    __builtin_amdgcn_wave_barrier();
-    if (in && (same >> lane) == 1) mine[d] = before + below + 1;   // the digit's last lane
-    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");         // (a wave's LDS accesses stay in order)
+    if (in && (same >> lane) == 1) seen[wave][d] = before + below + 1;   // the digit's last lane
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
   __syncthreads();
   for (int d = threadIdx.x; d < bins; d += 256) {
@@ -188,15 +241,133 @@ __global__ __launch_bounds__(256) void radix_scatter_kernel(key_source s, int64_
   }
 }
 
+// ---- the same order for short lists, in one launch ---------------------------------------------------------------------
+// An entry's place is the number of entries before it: those of a smaller key, and those of its own key that come earlier.
+// Every workgroup places 32 entries by comparing them with all n (staged in LDS, four keys a read, 32 slices of threads):
+// n^2 comparisons of two instructions each over the whole chip -- 6144 entries: 4.4 us against 25 us for the six launches of
+// two radix passes, which cost about the same at any short length (16384: 17 us).
+constexpr int kRankMax = 16384, kRankTokens = 32, kRankStage = 8192, kRankSlices = 1024 / kRankTokens;
+
+__global__ __launch_bounds__(1024) void rank_sort_kernel(key_source s, int n, uint32_t *__restrict__ keys_out,
+                                                         uint32_t *__restrict__ pos_out, uint32_t *__restrict__ n_crossing) {
+  __shared__ alignas(16) uint32_t stage[kRankStage];
+  __shared__ uint32_t part[kRankSlices][kRankTokens + 1];
+  if (blockIdx.x == 0 && threadIdx.x == 0) *n_crossing = 0;
+  const int i0 = blockIdx.x * kRankTokens, t = threadIdx.x % kRankTokens, slice = threadIdx.x / kRankTokens, i = i0 + t;
+  uint32_t own[1], pos[1], rank = 0, r4[4] = {0, 0, 0, 0};
+  load_keys<1>(s, i, 0, n, own, pos);
+  const uint32_t key = own[0];
+  for (int j0 = 0; j0 < n; j0 += kRankStage) {
+    constexpr int PER = kRankStage / 1024;
+    uint32_t k[PER], unused[PER];
+    load_keys<PER>(s, j0 + threadIdx.x, 1024, n, k, unused);
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < PER; ++e)                           // (behind the list: smaller than no key)
+      stage[e * 1024 + threadIdx.x] = j0 + e * 1024 + (int)threadIdx.x < n ? k[e] : 0xffffffffu;
+    __syncthreads();
+    // an earlier entry of the same key counts, a later one does not; the workgroup's own entries are taken as later ones
+    const int count = min(kRankStage, n - j0), mid = max(0, min(i0 - j0, count));
+    auto below = [&](int from, int to, uint32_t top) {
+#pragma unroll 4
+      for (int q = from + slice * 4; q < to; q += 4 * kRankSlices) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(&stage[q]);
+        r4[0] += v.x < top;                                 // (four chains: each step is a compare and an add with carry)
+        r4[1] += v.y < top;
+        r4[2] += v.z < top;
+        r4[3] += v.w < top;
+      }
+    };
+    below(0, mid, key + 1);
+    below(mid, count, key);
+    if (i0 >= j0 && i0 - j0 < kRankStage && slice < t && stage[i0 - j0 + slice] == key) ++rank;   // ... but for these
+  }
+  part[slice][t] = rank + r4[0] + r4[1] + r4[2] + r4[3];
+  __syncthreads();
+  if (threadIdx.x >= kRankTokens || i >= n) return;
+  uint32_t to = 0;
+#pragma unroll
+  for (int q = 0; q < kRankSlices; ++q) to += part[q][t];
+  keys_out[to] = key;
+  pos_out[to] = pos[0];
+}
+
 // ---- sums over the runs of equal ids ----------------------------------------------------------------------------------
-// GL lanes take `chunk` consecutive entries of the sorted list for their GL * VEC columns (blockIdx.y: the column block).
-// A run that lies inside the chunk is written to its row; a run that comes from the chunk before leaves its part in
-// slab[chunk][0], one that starts here and goes on in slab[chunk][1].
+// GL lanes take `chunk` consecutive entries of the sorted list for their GL * VEC columns (blockIdx.y: the column block),
+// eight rows on their way at a time.  A run that lies inside the chunk is written to its row; a run that comes from the
+// chunk before leaves its part in slab[chunk][0], one that starts here and goes on in slab[chunk][1], and is listed for the
+// launch behind (the list's order does not matter: its entries are independent of each other).
+// The blocks behind those of the chunks write the rows that no id names: zeros.  They wait on memory alone, the chunks'
+// blocks mostly on the latency of their rows, so the two share the launch.
+constexpr int kZeroRows = 64, kMarkMax = 16384;
+
+// First place in keys[lo, hi) that is not below `key`.
+__device__ __forceinline__ int64_t lower_bound(const uint32_t *__restrict__ keys, int64_t lo, int64_t hi, uint32_t key) {
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (keys[mid] < key) lo = mid + 1; else hi = mid;
+  }
+  return lo;
+}
+
+// The same by a whole wave, 64 probes a step.
+__device__ __forceinline__ int64_t wave_lower_bound(const uint32_t *__restrict__ keys, int64_t n, uint32_t key) {
+  int64_t lo = 0, hi = n;
+  const int lane = threadIdx.x & 63;
+  while (lo < hi) {
+    const int64_t step = (hi - lo + 63) >> 6, at = lo + lane * step;
+    const int below = __popcll(__ballot(at < hi && keys[at] < key));    // (the first ones: the keys ascend)
+    if (below == 0) return lo;
+    hi = min(hi, lo + below * step);
+    lo = lo + (below - 1) * step + 1;
+  }
+  return lo;
+}
+
+template <typename T, int VEC, int GL>
+__device__ __forceinline__ void zero_unnamed_rows(int64_t block, const uint32_t *__restrict__ keys, int64_t n, uint32_t n_rows, int dim,
+                                                  T *__restrict__ d_table) {
+  __shared__ uint8_t named[kZeroRows];
+  __shared__ int64_t ends[2];
+  const int64_t r0 = block * kZeroRows;
+  const int rows = (int)min((int64_t)kZeroRows, (int64_t)n_rows - r0);
+  if (threadIdx.x < kZeroRows) named[threadIdx.x] = 0;
+  if (threadIdx.x < 128) {
+    const int64_t at = wave_lower_bound(keys, n, (uint32_t)(r0 + (threadIdx.x >= 64 ? rows : 0)));
+    if ((threadIdx.x & 63) == 0) ends[threadIdx.x >> 6] = at;
+  }
+  __syncthreads();
+  const int64_t lo = ends[0], hi = ends[1];
+  if (hi - lo <= kMarkMax) {
+    for (int64_t i = lo + threadIdx.x; i < hi; i += 256) named[keys[i] - r0] = 1;
+  } else if ((int)threadIdx.x < rows) {                     // long runs: look for each row instead of reading them all
+    const uint32_t row = (uint32_t)r0 + threadIdx.x;
+    const int64_t at = lower_bound(keys, lo, hi, row);
+    named[threadIdx.x] = at < hi && keys[at] == row;
+  }
+  __syncthreads();
+  const int steps = dim / VEC, g = threadIdx.x / GL, l = threadIdx.x % GL;
+  float zero[VEC];
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) zero[v] = 0.f;
+  for (int r = g; r < rows; r += 256 / GL) {
+    if (named[r]) continue;
+    T *dst = d_table + (r0 + r) * dim;
+    for (int c = l; c < steps; c += GL) dg_store<VEC>(dst + c * VEC, zero);
+  }
+}
+
 template <typename T, int VEC, int GL>
 __global__ __launch_bounds__(256) void embedding_runs_kernel(const T *__restrict__ d_out, int64_t stride, int dim,
                                                              const uint32_t *__restrict__ keys, const uint32_t *__restrict__ pos,
-                                                             int64_t n, uint32_t n_rows, int chunk, float scale,
-                                                             T *__restrict__ d_table, float *__restrict__ slab) {
+                                                             int64_t n, uint32_t n_rows, int chunk, unsigned chunk_blocks, float scale,
+                                                             T *__restrict__ d_table, float *__restrict__ slab,
+                                                             uint32_t *__restrict__ crossing, uint32_t *__restrict__ n_crossing) {
+  if (blockIdx.x >= chunk_blocks) {
+    const int64_t block = (int64_t)(blockIdx.x - chunk_blocks) * gridDim.y + blockIdx.y;
+    if (block * kZeroRows < n_rows) zero_unnamed_rows<T, VEC, GL>(block, keys, n, n_rows, dim, d_table);
+    return;
+  }
   const int64_t c = (int64_t)blockIdx.x * (256 / GL) + threadIdx.x / GL;
   const int64_t b = c * chunk, e = min(b + chunk, n);
   if (b >= n) return;
@@ -211,6 +382,7 @@ __global__ __launch_bounds__(256) void embedding_runs_kernel(const T *__restrict
     if (!live || cur >= n_rows) return;
     if (open || goes_on) {
       dg_store<VEC>(slab + (size_t)(2 * c + (open ? 0 : 1)) * dim + col, acc);
+      if (!open && col == 0) crossing[atomicAdd(n_crossing, 1u)] = (uint32_t)c;
     } else {
       float f[VEC];
 #pragma unroll
@@ -218,16 +390,19 @@ __global__ __launch_bounds__(256) void embedding_runs_kernel(const T *__restrict
       dg_store<VEC>(d_table + (size_t)cur * dim + col, f);
     }
   };
-  constexpr int U = 4;
+  constexpr int U = 8;
   for (int64_t i = b; i < e; i += U) {
-    uint32_t k[U];
-    float row[U][VEC];
+    alignas(16) uint32_t k[U], p[U];          // (the lists reach to a multiple of 8 entries, whatever the ends hold)
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t j = min(i + u, e - 1);
-      k[u] = keys[j];
-      if (live) dg_load<VEC>(d_out + (int64_t)pos[j] * stride + col, row[u]);
+    for (int u = 0; u < U; u += 4) {
+      *reinterpret_cast<uint4 *>(k + u) = *reinterpret_cast<const uint4 *>(keys + i + u);
+      *reinterpret_cast<uint4 *>(p + u) = *reinterpret_cast<const uint4 *>(pos + i + u);
     }
+    if (k[0] >= n_rows) break;                // no gradient from here on
+    dg_vec<T, VEC> row[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (live && i + u < e) row[u] = dg_load_raw<VEC, 16>(d_out + (int64_t)p[u] * stride + col);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (i + u >= e) break;
@@ -240,85 +415,64 @@ __global__ __launch_bounds__(256) void embedding_runs_kernel(const T *__restrict
       }
       if (live) {
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) acc[v] += row[u][v];
+        for (int v = 0; v < VEC; ++v) acc[v] += dg_widen(row[u].v[v]);
       }
     }
   }
   flush(e < n && keys[e] == cur);
 }
 
-// First place in keys[0, n) that is not below `key`.
-__device__ __forceinline__ int64_t lower_bound(const uint32_t *__restrict__ keys, int64_t n, uint32_t key) {
-  int64_t lo = 0, hi = n;
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (keys[mid] < key) lo = mid + 1; else hi = mid;
-  }
-  return lo;
-}
-
-// Blocks [0, n_chunks): the run that starts in chunk c and goes on behind it -- its parts, chunk after chunk (256 / GL
-// strands of every so many chunks, added strand by strand).  The blocks behind them: rows that no id names become zero.
-constexpr int kZeroRows = 64;
-template <typename T, int VEC, int GL>
-__global__ __launch_bounds__(256) void embedding_finish_kernel(const uint32_t *__restrict__ keys, int64_t n, uint32_t n_rows, int dim,
-                                                               int chunk, int64_t n_chunks, float scale,
-                                                               const float *__restrict__ slab, T *__restrict__ d_table) {
-  __shared__ float part[256 / GL][GL * VEC];
-  __shared__ uint8_t named[kZeroRows];
-  if ((int64_t)blockIdx.x >= n_chunks) {
-    const int64_t r0 = ((int64_t)blockIdx.x - n_chunks) * kZeroRows;
-    if (threadIdx.x < kZeroRows) {
-      const int64_t row = r0 + threadIdx.x;
-      bool is = true;
-      if (row < n_rows) {
-        const int64_t at = lower_bound(keys, n, (uint32_t)row);
-        is = at < n && keys[at] == (uint32_t)row;
+// The runs that cross from chunk to chunk, 64 columns of one at a time: 16 strands of every 16th part, the strands added in
+// order.  A workgroup takes every so many of them from the list.
+constexpr int kCrossCols = 64;
+template <typename T>
+__global__ __launch_bounds__(256) void embedding_crossing_kernel(const uint32_t *__restrict__ keys, int64_t n, int dim, int chunk,
+                                                                 float scale, const float *__restrict__ slab,
+                                                                 const uint32_t *__restrict__ crossing,
+                                                                 const uint32_t *__restrict__ n_crossing, T *__restrict__ d_table) {
+  __shared__ float part[16][kCrossCols];
+  __shared__ int64_t last_chunk;
+  const int64_t blocks = (dim + kCrossCols - 1) / kCrossCols, items = (int64_t)*n_crossing * blocks;
+  const int g = threadIdx.x >> 4, l = threadIdx.x & 15;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int64_t c = crossing[item / blocks];
+    const int col = (int)(item % blocks) * kCrossCols + 4 * l;
+    const uint32_t key = keys[(c + 1) * chunk];             // (it goes on there)
+    __syncthreads();
+    if (threadIdx.x < 64) {                                 // the last chunk that begins with the run
+      int64_t last = c + 1;
+      for (;;) {
+        const int64_t j = last + 1 + (threadIdx.x & 63);
+        const int more = __popcll(__ballot(j * chunk < n && keys[min(j * chunk, n - 1)] == key));
+        last += more;
+        if (more < 64) break;
       }
-      named[threadIdx.x] = is;
+      if (threadIdx.x == 0) last_chunk = last;
     }
     __syncthreads();
-    const int steps = (dim + VEC - 1) / VEC;
-    float zero[VEC];
+    const int64_t last = last_chunk;
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int64_t k = c + g; k <= last; k += 16) {
+      const float *src = slab + (size_t)(2 * k + (k == c ? 1 : 0)) * dim + col;
+      if (col + 4 <= dim) {
+        float f[4];
+        dg_load_unaligned<4>(src, f);
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) zero[v] = 0.f;
-    for (int64_t q = threadIdx.x; q < (int64_t)kZeroRows * steps; q += 256) {
-      const int r = (int)(q / steps), c = (int)(q % steps) * VEC;
-      if (!named[r]) dg_store<VEC>(d_table + (r0 + r) * dim + c, zero);
-    }
-    return;
-  }
-  const int64_t c = blockIdx.x, b = c * chunk, e = min(b + chunk, n);
-  const uint32_t key = keys[e - 1];
-  if (key >= n_rows || e >= n || keys[e] != key) return;             // nothing goes on behind this chunk
-  if (keys[b] == key && b > 0 && keys[b - 1] == key) return;         // ... or it began before it
-  const int64_t end = lower_bound(keys, n, key + 1), last = (end - 1) / chunk;
-  const int g = threadIdx.x / GL, l = threadIdx.x % GL;
-  for (int c0 = 0; c0 < dim; c0 += GL * VEC) {
-    const int col = c0 + l * VEC;
-    float acc[VEC];
+        for (int v = 0; v < 4; ++v) acc[v] += f[v];
+      } else {
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) acc[v] = 0.f;
-    if (col < dim) {
-      for (int64_t k = c + g; k <= last; k += 256 / GL) {
-        float f[VEC];
-        dg_load<VEC>(slab + (size_t)(2 * k + (k == c ? 1 : 0)) * dim + col, f);
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) acc[v] += f[v];
+        for (int v = 0; v < 4; ++v)
+          if (col + v < dim) acc[v] += src[v];
       }
     }
-    __syncthreads();
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) part[g][l * VEC + v] = acc[v];
+    for (int v = 0; v < 4; ++v) part[g][4 * l + v] = acc[v];
     __syncthreads();
-    if (g == 0 && col < dim) {
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        float t = part[0][l * VEC + v];
-        for (int k = 1; k < 256 / GL; ++k) t += part[k][l * VEC + v];
-        acc[v] = t * scale;
-      }
-      dg_store<VEC>(d_table + (size_t)key * dim + col, acc);
+    const int o = (int)(item % blocks) * kCrossCols + threadIdx.x;
+    if (threadIdx.x < kCrossCols && o < dim) {
+      float t = part[0][threadIdx.x];
+      for (int q = 1; q < 16; ++q) t += part[q][threadIdx.x];
+      d_table[(size_t)key * dim + o] = dg_round<T>(t * scale);
     }
   }
 }
@@ -330,14 +484,15 @@ int items_per_thread(int64_t n) { return n <= 256 * 256 * 4 ? 4 : kMaxIpt; }
 // Entries of a chunk: short ones while the list is short (every CU gets some), longer ones as it grows.
 int chunk_of(int64_t n, int dim) {
   int c = 8;
-  while (c < 256 && n / c > 4096) c <<= 1;
+  while (c < 256 && n / c > 2048) c <<= 1;
   return c;
 }
 
 struct grad_plan {
   int64_t n_blocks, n_chunks;
   int ipt, chunk, passes, bits;     // bits of the id's range
-  size_t keys, pos, counts, totals, slab, bytes;   // offsets (two key and position lists)
+  bool ranked;
+  size_t keys, pos, counts, totals, crossing, slab, bytes;   // offsets (two key and position lists)
 };
 
 grad_plan plan_of(int64_t n_ids, int64_t n_rows, int dim) {
@@ -349,12 +504,15 @@ grad_plan plan_of(int64_t n_ids, int64_t n_rows, int dim) {
   p.bits = 1;
   while (p.bits < 32 && (n_rows >> p.bits) != 0) ++p.bits;     // keys 0 .. n_rows
   p.passes = (p.bits + kMaxDigit - 1) / kMaxDigit;
-  const size_t list = ((size_t)n_ids * 4 + 255) & ~(size_t)255;
+  p.ranked = n_ids <= kRankMax;
+  const size_t list = ((size_t)n_ids * 4 + 255) & ~(size_t)255;   // (a multiple of 8 entries)
   size_t at = 0;
-  p.keys = at; at += 2 * list;
-  p.pos = at; at += 2 * list;
-  p.counts = at; at += (((size_t)p.n_blocks << kMaxDigit) * 4 + 255) & ~(size_t)255;
-  p.totals = at; at += (size_t)4 << kMaxDigit;
+  const int lists = p.ranked ? 1 : 2;
+  p.keys = at; at += lists * list;
+  p.pos = at; at += lists * list;
+  p.counts = at; at += p.ranked ? 0 : (((size_t)p.n_blocks << kMaxDigit) * 4 + 255) & ~(size_t)255;
+  p.totals = at; at += p.ranked ? 0 : (size_t)4 << kMaxDigit;
+  p.crossing = at; at += ((size_t)p.n_chunks * 4 + 4 + 255) & ~(size_t)255;    // their number, then the chunks
   p.slab = at; at += (size_t)p.n_chunks * 2 * dim * 4;
   p.bytes = at;
   return p;
@@ -379,17 +537,18 @@ int lookup_as(const void *table, int64_t n_rows, int64_t stride, int dim, const 
 
 template <typename T, int VEC, int GL>
 int grad_as(const grad_plan &p, const void *d_out, int64_t stride, const uint32_t *keys, const uint32_t *pos, int64_t n, int64_t n_rows,
-            int dim, float scale, void *d_table, float *slab, hipStream_t stream) {
-  if (n > 0) {
-    const int64_t blocks = (p.n_chunks + 256 / GL - 1) / (256 / GL);
-    const int cols = (dim + GL * VEC - 1) / (GL * VEC);
-    hipLaunchKernelGGL((embedding_runs_kernel<T, VEC, GL>), dim3((unsigned)blocks, cols), dim3(256), 0, stream, (const T *)d_out, stride,
-                       dim, keys, pos, n, (uint32_t)n_rows, p.chunk, scale, (T *)d_table, slab);
-    DG_HIP(hipGetLastError());
-  }
-  const int64_t blocks = p.n_chunks + (n_rows + kZeroRows - 1) / kZeroRows;
-  hipLaunchKernelGGL((embedding_finish_kernel<T, VEC, GL>), dim3((unsigned)blocks), dim3(256), 0, stream, keys, n, (uint32_t)n_rows, dim,
-                     p.chunk, p.n_chunks, scale, slab, (T *)d_table);
+            int dim, float scale, void *d_table, float *slab, uint32_t *crossing, hipStream_t stream) {
+  const unsigned chunk_blocks = (unsigned)((p.n_chunks + 256 / GL - 1) / (256 / GL));
+  const int cols = (dim + GL * VEC - 1) / (GL * VEC);
+  const int64_t zero_blocks = (n_rows + kZeroRows - 1) / kZeroRows;
+  const dim3 grid(chunk_blocks + (unsigned)((zero_blocks + cols - 1) / cols), cols);
+  hipLaunchKernelGGL((embedding_runs_kernel<T, VEC, GL>), grid, dim3(256), 0, stream, (const T *)d_out, stride, dim, keys, pos, n,
+                     (uint32_t)n_rows, p.chunk, chunk_blocks, scale, (T *)d_table, slab, crossing + 1, crossing);
+  DG_HIP(hipGetLastError());
+  if (p.n_chunks < 2) return 0;      // nothing to cross into
+  const int64_t items = p.n_chunks * ((dim + kCrossCols - 1) / kCrossCols);
+  hipLaunchKernelGGL((embedding_crossing_kernel<T>), dim3((unsigned)(items < 2048 ? items : 2048)), dim3(256), 0, stream, keys, n, dim,
+                     p.chunk, scale, slab, crossing + 1, crossing, (T *)d_table);
   DG_HIP(hipGetLastError());
   return 0;
 }
@@ -453,25 +612,29 @@ extern "C" int dg_embedding_grad(const void *d_out, int64_t row_stride, const vo
     return dg_fail(DG_ERR_SIZE, "dg_embedding_grad: a 16-byte aligned workspace of %zu bytes is needed, got %zu", p.bytes, workspace_bytes);
   hipStream_t st = (hipStream_t)stream;
   char *ws = (char *)workspace;
-  const size_t list = (p.pos - p.keys) / 2;
+  const size_t list = p.ranked ? 0 : (p.pos - p.keys) / 2;
   uint32_t *keys[2] = {(uint32_t *)(ws + p.keys), (uint32_t *)(ws + p.keys + list)};
   uint32_t *pos[2] = {(uint32_t *)(ws + p.pos), (uint32_t *)(ws + p.pos + list)};
   uint32_t *counts = (uint32_t *)(ws + p.counts), *totals = (uint32_t *)(ws + p.totals);
+  uint32_t *crossing = (uint32_t *)(ws + p.crossing);
   int at = 0;
-  if (n_ids) {
+  if (n_ids && p.ranked) {
+    const key_source s = {ids, ids_are_64, padding_idx, (uint32_t)n_rows, nullptr, nullptr};
+    hipLaunchKernelGGL(rank_sort_kernel, dim3((unsigned)((n_ids + kRankTokens - 1) / kRankTokens)), dim3(1024), 0, st, s, (int)n_ids, keys[0],
+                       pos[0], crossing);
+    DG_HIP(hipGetLastError());
+  } else if (n_ids) {
     key_source s = {ids, ids_are_64, padding_idx, (uint32_t)n_rows, nullptr, nullptr};
     for (int pass = 0, shift = 0; pass < p.passes; ++pass) {
       const int bits = (p.bits - shift + (p.passes - pass) - 1) / (p.passes - pass);
       const dim3 grid((unsigned)p.n_blocks);
-      if (p.ipt == 4)
-        hipLaunchKernelGGL((radix_count_kernel<4>), grid, dim3(256), 0, st, s, n_ids, shift, bits, (int)p.n_blocks, counts);
-      else
-        hipLaunchKernelGGL((radix_count_kernel<kMaxIpt>), grid, dim3(256), 0, st, s, n_ids, shift, bits, (int)p.n_blocks, counts);
-      hipLaunchKernelGGL(radix_scan_kernel, dim3(1u << bits), dim3(256), 0, st, counts, (int)p.n_blocks, totals);
-      if (p.ipt == 4)
-        hipLaunchKernelGGL((radix_scatter_kernel<4>), grid, dim3(256), 0, st, s, n_ids, shift, bits, (int)p.n_blocks, counts, totals, keys[at], pos[at]);
-      else
-        hipLaunchKernelGGL((radix_scatter_kernel<kMaxIpt>), grid, dim3(256), 0, st, s, n_ids, shift, bits, (int)p.n_blocks, counts, totals, keys[at], pos[at]);
+      const int nb = (int)p.n_blocks, by_block = nb <= kSelfScan;
+      const uint32_t *sums = by_block ? nullptr : totals;
+      if (p.ipt == 4) hipLaunchKernelGGL((radix_count_kernel<4>), grid, dim3(256), 0, st, s, n_ids, shift, bits, nb, by_block, counts, crossing);
+      else hipLaunchKernelGGL((radix_count_kernel<kMaxIpt>), grid, dim3(256), 0, st, s, n_ids, shift, bits, nb, by_block, counts, crossing);
+      if (!by_block) hipLaunchKernelGGL(radix_scan_kernel, dim3(1u << bits), dim3(256), 0, st, counts, nb, totals);
+      if (p.ipt == 4) hipLaunchKernelGGL((radix_scatter_kernel<4>), grid, dim3(256), 0, st, s, n_ids, shift, bits, nb, counts, sums, keys[at], pos[at]);
+      else hipLaunchKernelGGL((radix_scatter_kernel<kMaxIpt>), grid, dim3(256), 0, st, s, n_ids, shift, bits, nb, counts, sums, keys[at], pos[at]);
       DG_HIP(hipGetLastError());
       s.keys = keys[at];
       s.pos = pos[at];
@@ -483,5 +646,5 @@ extern "C" int dg_embedding_grad(const void *d_out, int64_t row_stride, const vo
   const int z = type_size(dtype);
   const bool wide = (!n_ids || aligned(d_out, row_stride, dim, z)) && aligned(d_table, dim, dim, z);
   DG_BY_TYPE(grad_as, dtype, wide, dim, p, d_out, row_stride, keys[at], pos[at], n_ids, n_rows, dim, scale, d_table,
-             (float *)(ws + p.slab), st)
+             (float *)(ws + p.slab), crossing, st)
 }

@@ -1010,13 +1010,11 @@ def embedding_lookup(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0)
     if n < 1 and ids.numel():
         raise DiffGraphHipError("table: has no rows to look up")
     dev = table.device
-    with _lib.on_device(dev):
-        out = torch.empty((*ids.shape, dim), dtype=table.dtype, device=dev)
-        if out.numel():
-            rc = _lib.load().dg_embedding_lookup(table.data_ptr(), n, table.stride(0), dim, _ELEMENT[table.dtype], ids.data_ptr(),
-                                                 int(ids.dtype == torch.int64), ids.numel(), float(scale), out.data_ptr(),
-                                                 _lib.stream_ptr(dev))
-            _lib.check(rc, "dg_embedding_lookup")
+    out = torch.empty((*ids.shape, dim), dtype=table.dtype, device=dev)
+    count = ids.numel()
+    if count:
+        _lib.launch(dev, _lib.load().dg_embedding_lookup, "dg_embedding_lookup", table.data_ptr(), n, table.stride(0), dim,
+                    _ELEMENT[table.dtype], ids.data_ptr(), ids.dtype == torch.int64, count, scale, out.data_ptr())
     return out
 
 
@@ -1039,14 +1037,11 @@ def embedding_grad(d_out: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: f
     if padding_idx is not None and not 0 <= padding_idx < n_rows:
         raise DiffGraphHipError(f"padding_idx must lie in [0,{n_rows}); got {padding_idx}")
     lib, n = _lib.load(), ids.numel()
-    with _lib.on_device(dev):
-        grad = torch.empty((n_rows, dim), dtype=d.dtype, device=dev)
-        ws_bytes = int(lib.dg_embedding_grad_workspace(n, n_rows, dim)) if n else 0
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-        rc = lib.dg_embedding_grad(d.data_ptr(), d.stride(0), ids.data_ptr(), int(ids.dtype == torch.int64), n, n_rows, dim,
-                                   _ELEMENT[d.dtype], float(scale), -1 if padding_idx is None else int(padding_idx),
-                                   grad.data_ptr(), ws.data_ptr(), ws_bytes, _lib.stream_ptr(dev))
-        _lib.check(rc, "dg_embedding_grad")
+    grad = torch.empty((n_rows, dim), dtype=d.dtype, device=dev)
+    ws_bytes = lib.dg_embedding_grad_workspace(n, n_rows, dim) if n else 0
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    _lib.launch(dev, lib.dg_embedding_grad, "dg_embedding_grad", d.data_ptr(), d.stride(0), ids.data_ptr(), ids.dtype == torch.int64, n,
+                n_rows, dim, _ELEMENT[d.dtype], scale, -1 if padding_idx is None else padding_idx, grad.data_ptr(), ws.data_ptr(), ws_bytes)
     return grad
 
 
@@ -1152,8 +1147,7 @@ def adjust_scores(scores: torch.Tensor, *, history=None, rows: Optional[torch.Te
     elif allowed_rows is not None:
         raise DiffGraphHipError("allowed: allowed_rows needs masks")
     if n and items:
-        with _lib.on_device(dev):
-            _lib.check(_lib.load().dg_adjust_scores(C.byref(t), _lib.stream_ptr(dev)), "dg_adjust_scores")
+        _lib.launch(dev, _lib.load().dg_adjust_scores, "dg_adjust_scores", C.byref(t))
     return out
 
 
@@ -1178,11 +1172,9 @@ class Checkpoint8:
             raise DiffGraphHipError(f"values: float32, bfloat16 or float16, not {dtype}")
         n, k = self.shape
         dev = self.codes.device
-        with _lib.on_device(dev):
-            out = torch.empty((n, k), dtype=dtype, device=dev)
-            rc = _lib.load().dg_checkpoint8_values(self.codes.data_ptr(), self.scales.data_ptr(), n, k, _FORMATS[self.format],
-                                                   _ELEMENT[dtype], out.data_ptr(), _lib.stream_ptr(dev))
-            _lib.check(rc, "dg_checkpoint8_values")
+        out = torch.empty((n, k), dtype=dtype, device=dev)
+        _lib.launch(dev, _lib.load().dg_checkpoint8_values, "dg_checkpoint8_values", self.codes.data_ptr(), self.scales.data_ptr(), n, k,
+                    _FORMATS[self.format], _ELEMENT[dtype], out.data_ptr())
         return out
 
     def check(self, name: str, n: int, device) -> None:
@@ -1204,12 +1196,10 @@ def checkpoint8(x: torch.Tensor, format: str = "int8") -> Checkpoint8:
         raise DiffGraphHipError(f"format: 'int8' or 'e4m3', got {format!r}")
     n, k = x.shape
     dev = x.device
-    with _lib.on_device(dev):
-        codes = torch.empty((n, (k + 15) // 16 * 16), dtype=torch.uint8, device=dev)
-        scales = torch.empty((n, (k + 31) // 32), dtype=torch.uint8, device=dev)
-        rc = _lib.load().dg_checkpoint8(x.data_ptr(), x.stride(0), n, k, _ELEMENT[x.dtype], _FORMATS[format], codes.data_ptr(),
-                                        scales.data_ptr(), _lib.stream_ptr(dev))
-        _lib.check(rc, "dg_checkpoint8")
+    codes = torch.empty((n, (k + 15) // 16 * 16), dtype=torch.uint8, device=dev)
+    scales = torch.empty((n, (k + 31) // 32), dtype=torch.uint8, device=dev)
+    _lib.launch(dev, _lib.load().dg_checkpoint8, "dg_checkpoint8", x.data_ptr(), x.stride(0), n, k, _ELEMENT[x.dtype], _FORMATS[format],
+                codes.data_ptr(), scales.data_ptr())
     return Checkpoint8(codes, scales, (n, k), format)
 
 
@@ -1227,15 +1217,12 @@ def checkpoint8_backward(d_y: torch.Tensor, x: Checkpoint8, y: Optional[Checkpoi
         if y.shape[1] != m or y.format != x.format:
             raise DiffGraphHipError(f"y: expected {m} columns in the format of x ({x.format})")
     lib = _lib.load()
-    with _lib.on_device(dev):
-        ws_bytes = int(lib.dg_checkpoint8_backward_workspace(n, k, m))
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-        d_z = d_y if y is None else torch.empty((n, m), dtype=d_y.dtype, device=dev)
-        d_w = torch.empty((m, k), dtype=d_y.dtype, device=dev)
-        d_b = torch.empty(m, dtype=d_y.dtype, device=dev)
-        rc = lib.dg_checkpoint8_backward(d_y.data_ptr(), d_y.stride(0), n, m, k, _ELEMENT[d_y.dtype], _FORMATS[x.format],
-                                         x.codes.data_ptr(), x.scales.data_ptr(), None if y is None else y.codes.data_ptr(),
-                                         None if y is None else y.scales.data_ptr(), d_z.data_ptr(), d_w.data_ptr(), d_b.data_ptr(),
-                                         ws.data_ptr(), ws_bytes, _lib.stream_ptr(dev))
-        _lib.check(rc, "dg_checkpoint8_backward")
+    ws_bytes = lib.dg_checkpoint8_backward_workspace(n, k, m)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    d_z = d_y if y is None else torch.empty((n, m), dtype=d_y.dtype, device=dev)
+    d_w = torch.empty((m, k), dtype=d_y.dtype, device=dev)
+    d_b = torch.empty(m, dtype=d_y.dtype, device=dev)
+    _lib.launch(dev, lib.dg_checkpoint8_backward, "dg_checkpoint8_backward", d_y.data_ptr(), d_y.stride(0), n, m, k, _ELEMENT[d_y.dtype],
+                _FORMATS[x.format], x.codes.data_ptr(), x.scales.data_ptr(), None if y is None else y.codes.data_ptr(),
+                None if y is None else y.scales.data_ptr(), d_z.data_ptr(), d_w.data_ptr(), d_b.data_ptr(), ws.data_ptr(), ws_bytes)
     return d_z, d_w, d_b
