@@ -133,7 +133,6 @@ struct back_args {
   int x_pitch, x_groups, y_pitch, y_groups;
   int64_t n;
   int k, m;
-  int64_t rows_per_strip;
   int strips, tiles_m, tiles_n;
   void *d_z;            // contiguous [n][m], written under tanh
   float *part, *part_b; // [strip][tile_m][tile_n][BM][BN], [strip][tiles_m * BM]
@@ -143,33 +142,54 @@ __device__ __forceinline__ uint32_t high_halves(float a, float b) {   // bf16(a)
   return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
 }
 
-// A workgroup sums one strip of rows for a BM x BN tile of d_w, BK rows at a time: its threads load quads of rows x quads
-// of columns, form d_z, cut it, and lay both operands down in LDS with eight rows of a column in 16 bytes -- what a lane
-// of the matrix instruction takes -- transposing in their registers.  A column c sits in slot (c mod 4) (B / 4) + c / 4, so
-// that neighbouring lanes write neighbouring slots; results are kept in slot order until the second launch.
-// The next rows are on their way while the matrix instructions run.
-template <typename T, int FMT, bool TANH, int PIECES, int BM, int BN>
+// What a thread holds of a step's operands until it lays them down: four rows of WA columns of d_y (and of the codes of
+// y), four rows of WB columns of the codes of x, each row with its group's scale byte.
+template <typename T, int WA, int WB>
+struct back_regs {
+  dg_vec<T, WA> d[4];
+  uint32_t yw[4], ys[4], xw[4], xs[4];
+};
+
+// W neighbouring codes at p (W = 2 or 4; p a multiple of W).
+template <int W>
+__device__ __forceinline__ uint32_t load_codes(const uint8_t *p) {
+  if constexpr (W == 4) return *reinterpret_cast<const uint32_t *>(p);
+  return *reinterpret_cast<const uint16_t *>(p);
+}
+
+// A workgroup sums one strip of rows -- every so many blocks of 32, so that all workgroups together read on through the
+// memory -- for a BM x BN tile of d_w, a block a step: its threads load quads of rows x a few
+// columns, form d_z, cut it, and lay both operands down in LDS with eight rows of a column in 16 bytes -- what a lane of
+// the matrix instruction takes -- transposing in their registers.  A column c of a tile of B sits in slot
+// (c mod W) 32 + c / W, W = B / 32, so that neighbouring lanes write neighbouring slots; results are kept in slot order
+// until the second launch.  Two buffers in LDS and a step on its way in registers: one barrier a step, and the conversion of
+// the next step runs beside the matrix instructions of this one.
+// NARROW: d_y has one column (a load of two would leave its row).
+template <typename T, int FMT, bool TANH, int PIECES, int BM, int BN, bool NARROW>
 __global__ __launch_bounds__(256) void checkpoint8_backward_kernel(back_args a) {
-  constexpr int BK = BM == 128 && BN == 128 ? 32 : 64, WM = BM / 2, WN = BN / 2, TM = WM / 32, TN = WN / 32;
-  constexpr int UA = BM * BK / 16 / 256, UB = BN * BK / 16 / 256;      // 4 x 4 units per thread and step
-  __shared__ u32x4 lds_a[PIECES][BK / 8][BM], lds_b[BK / 8][BN];
-  __shared__ float col_sums[BK / 4][BM];
+  constexpr int BK = 32, WA = BM / 32, WB = BN / 32, WM = BM / 2, WN = BN / 2, TM = WM / 32, TN = WN / 32;
+  struct buffer {
+    u32x4 a[PIECES][BK / 8][BM], b[BK / 8][BN];
+  };
+  __shared__ buffer lds[2];
   const int tiles = a.tiles_m * a.tiles_n;
   const int xcd = blockIdx.x & 7, idx = blockIdx.x >> 3;               // the tiles of a strip share an L2
   const int strip = idx / tiles * 8 + xcd, tile = idx % tiles;
   if (strip >= a.strips) return;
   const int m0 = tile / a.tiles_n * BM, n0 = tile % a.tiles_n * BN;
   const bool first_n = n0 == 0;
-  const int64_t r0 = (int64_t)strip * a.rows_per_strip, r1 = min(r0 + a.rows_per_strip, a.n);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = (wave >> 1) * WM, wn = (wave & 1) * WN;
+  const int cw = tid & 31, rq = tid >> 5, steps = (int)(((a.n + BK - 1) / BK - strip + a.strips - 1) / a.strips);
+  // columns behind the last one: some other column's values, in rows or columns of the tile that nobody keeps
+  const int ca = min(m0 + cw * WA, a.m - 1) / WA * WA, cb = min(n0 + cw * WB, a.k - 1) / WB * WB;
+  const int ga = ca / kGroup, gb = cb / kGroup;
+  // the last columns of an odd width are read from further left, and moved into place when they are laid down
+  const bool odd = a.m % WA != 0;
+  const int from = odd && !NARROW ? min(ca, a.m - WA) : ca, shift = ca - from;
 
-  float d[UA][4][4];
-  uint32_t yw[UA][4], ys[UA][4], xw[UB][4], xs[UB][4];
-  float sums[UA][4];
+  float sums[WA];
 #pragma unroll
-  for (int u = 0; u < UA; ++u)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) sums[u][j] = 0.f;
+  for (int j = 0; j < WA; ++j) sums[j] = 0.f;
   f32x16 acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
@@ -178,122 +198,126 @@ __global__ __launch_bounds__(256) void checkpoint8_backward_kernel(back_args a) 
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
-  auto fetch = [&](int64_t base) {
+  auto fetch = [&](back_regs<T, WA, WB> &g, int step) {
+    const int64_t base = ((int64_t)min(step, steps - 1) * a.strips + strip) * BK;      // (no branch: the loads stay countable)
+    const int left = (int)min((int64_t)BK, a.n - base);
+    const T *dy = (const T *)a.d_y + base * a.d_stride;                // (uniform; a lane's part fits 32 bits)
+    const uint8_t *x = a.x + base * a.x_pitch, *xs = a.x_scales + base * a.x_groups;
+    const uint8_t *y = a.y + base * a.y_pitch, *ys = a.y_scales + base * a.y_groups;
 #pragma unroll
-    for (int u = 0; u < UA; ++u) {
-      const int unit = tid + 256 * u, c = m0 + unit % (BM / 4) * 4;
-      const int64_t row = base + unit / (BM / 4) * 4;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const bool in = row + q < r1 && c < a.m;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) d[u][q][j] = 0.f;
-        if (TANH) yw[u][q] = ys[u][q] = 0;
-        if (!in) continue;
-        const T *src = (const T *)a.d_y + (row + q) * a.d_stride + c;
-        if (c + 4 <= a.m) {
-          dg_load_unaligned<4>(src, d[u][q]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (c + j < a.m) d[u][q][j] = dg_widen(src[j]);
-        }
-        if (TANH) {
-          yw[u][q] = *reinterpret_cast<const uint32_t *>(a.y + (row + q) * a.y_pitch + c);
-          ys[u][q] = a.y_scales[(row + q) * a.y_groups + c / kGroup];
-        }
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < UB; ++u) {
-      const int unit = tid + 256 * u, c = n0 + unit % (BN / 4) * 4;
-      const int64_t row = base + unit / (BN / 4) * 4;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        xw[u][q] = xs[u][q] = 0;
-        if (row + q < r1 && c < a.k) {
-          xw[u][q] = *reinterpret_cast<const uint32_t *>(a.x + (row + q) * a.x_pitch + c);
-          xs[u][q] = a.x_scales[(row + q) * a.x_groups + c / kGroup];
-        }
-      }
-    }
-  };
-
-  auto lay_down = [&](int64_t base) {
-#pragma unroll
-    for (int u = 0; u < UA; ++u) {
-      const int unit = tid + 256 * u, c4 = unit % (BM / 4), rq = unit / (BM / 4), c = m0 + c4 * 4;
+    for (int q = 0; q < 4; ++q) {
+      const uint32_t r = min(rq * 4 + q, left - 1);                    // (rows behind the strip: cleared when laid down)
+      const T *src = dy + (r * (uint32_t)a.d_stride + from);
+      if constexpr (!NARROW) g.d[q] = dg_load_raw<WA, 2>(src);
+      else g.d[q].v[0] = g.d[q].v[1] = *src;
       if (TANH) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float y[4];
-          decode4<FMT>(yw[u][q], ys[u][q], y);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) d[u][q][j] *= 1.f - y[j] * y[j];
-          const int64_t row = base + rq * 4 + q;
-          if (first_n && row < r1 && c < a.m) {
-            T *dst = (T *)a.d_z + row * a.m + c;
-            if (c + 4 <= a.m) {
-              dg_store_unaligned<4>(dst, d[u][q]);
-            } else {
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (c + j < a.m) dst[j] = dg_round<T>(d[u][q][j]);
-            }
-          }
-        }
+        g.yw[q] = load_codes<WA>(y + (r * (uint32_t)a.y_pitch + ca));
+        g.ys[q] = ys[r * (uint32_t)a.y_groups + ga];
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float v[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] = d[u][q][j];
-        sums[u][j] += (v[0] + v[1]) + (v[2] + v[3]);
-#pragma unroll
-        for (int p = 0; p < PIECES; ++p) {
-          const u32x2 w = {high_halves(v[0], v[1]), high_halves(v[2], v[3])};
-          reinterpret_cast<u32x2 *>(&lds_a[p][rq >> 1][j * (BM / 4) + c4])[rq & 1] = w;
-          if (p + 1 < PIECES) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) v[q] -= __uint_as_float(__float_as_uint(v[q]) & 0xffff0000u);   // (exact)
-          }
-        }
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < UB; ++u) {
-      const int unit = tid + 256 * u, c4 = unit % (BN / 4), rq = unit / (BN / 4);
-      float v[4][4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) decode4<FMT>(xw[u][q], xs[u][q], v[q]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const u32x2 w = {high_halves(v[0][j], v[1][j]), high_halves(v[2][j], v[3][j])};
-        reinterpret_cast<u32x2 *>(&lds_b[rq >> 1][j * (BN / 4) + c4])[rq & 1] = w;
-      }
+      g.xw[q] = load_codes<WB>(x + (r * (uint32_t)a.x_pitch + cb));
+      g.xs[q] = xs[r * (uint32_t)a.x_groups + gb];
     }
   };
 
-  fetch(r0);
-  for (int64_t base = r0; base < r1; base += BK) {
-    lay_down(base);
-    __syncthreads();
-    if (base + BK < r1) fetch(base + BK);
+  auto lay_down = [&](back_regs<T, WA, WB> &g, int step, buffer &to) {
+    const int64_t base = ((int64_t)step * a.strips + strip) * BK;
+    const int left = step < steps ? (int)min((int64_t)BK, a.n - base) : 0;   // (rows behind the last one: zeros, by selection)
+    float d[4][WA];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+#pragma unroll
+      for (int j = 0; j < WA; ++j) d[q][j] = dg_widen(g.d[q].v[j]);
+#pragma unroll
+      for (int by = WA / 2; by; by >>= 1)
+#pragma unroll
+        for (int j = 0; j + by < WA; ++j) {
+          const float here = d[q][j], there = d[q][j + by];
+          d[q][j] = (shift & by) ? there : here;
+        }
+    }
+    if (TANH) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float y[4];
+        decode4<FMT>(g.yw[q], g.ys[q], y);
+#pragma unroll
+        for (int j = 0; j < WA; ++j) d[q][j] *= 1.f - y[j] * y[j];
+        if (first_n && rq * 4 + q < left && m0 + cw * WA < a.m) {
+          T *dst = (T *)a.d_z + (base + rq * 4 + q) * a.m + ca;
+          if (!odd) {
+            dg_store_unaligned<WA>(dst, d[q]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < WA; ++j)
+              if (ca + j < a.m) dst[j] = dg_round<T>(d[q][j]);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const bool in = rq * 4 + q < left;
+#pragma unroll
+      for (int j = 0; j < WA; ++j) d[q][j] = in ? d[q][j] : 0.f;
+      g.xs[q] = in ? g.xs[q] : 0;
+    }
+    if (first_n) {
+#pragma unroll
+      for (int j = 0; j < WA; ++j) sums[j] += (d[0][j] + d[1][j]) + (d[2][j] + d[3][j]);
+    }
+#pragma unroll
+    for (int j = 0; j < WA; ++j) {
+      float v[4] = {d[0][j], d[1][j], d[2][j], d[3][j]};
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p) {
+        u32x2 w;
+        w = {high_halves(v[0], v[1]), high_halves(v[2], v[3])};
+        reinterpret_cast<u32x2 *>(&to.a[p][rq >> 1][j * 32 + cw])[rq & 1] = w;
+        if (p + 1 < PIECES) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) v[q] -= __uint_as_float(__float_as_uint(v[q]) & 0xffff0000u);   // (exact)
+        }
+      }
+    }
+    float x[4][4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) decode4<FMT>(g.xw[q], g.xs[q], x[q]);
+#pragma unroll
+    for (int j = 0; j < WB; ++j) {
+      const u32x2 w = {high_halves(x[0][j], x[1][j]), high_halves(x[2][j], x[3][j])};
+      reinterpret_cast<u32x2 *>(&to.b[rq >> 1][j * 32 + cw])[rq & 1] = w;
+    }
+  };
+
+  auto multiply = [&](const buffer &from) {
 #pragma unroll
     for (int kk = 0; kk < BK / 16; ++kk) {
       const int k8 = kk * 2 + (lane >> 5);
       bf16x8 fb[TN];
 #pragma unroll
-      for (int j = 0; j < TN; ++j) fb[j] = __builtin_bit_cast(bf16x8, lds_b[k8][wn + j * 32 + (lane & 31)]);
+      for (int j = 0; j < TN; ++j) fb[j] = __builtin_bit_cast(bf16x8, from.b[k8][wn + j * 32 + (lane & 31)]);
 #pragma unroll
       for (int p = 0; p < PIECES; ++p)
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
-          const bf16x8 fa = __builtin_bit_cast(bf16x8, lds_a[p][k8][wm + i * 32 + (lane & 31)]);
+          const bf16x8 fa = __builtin_bit_cast(bf16x8, from.a[p][k8][wm + i * 32 + (lane & 31)]);
 #pragma unroll
           for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa, fb[j], acc[i][j], 0, 0, 0);
         }
     }
+  };
+
+  // Step i is multiplied out of buffer i mod 2 while step i + 1 is laid down in the other and step i + 2 is asked for.
+  // Steps behind the last one are zeros: no branch round a load.
+  back_regs<T, WA, WB> g;
+  fetch(g, 0);
+  lay_down(g, 0, lds[0]);
+  fetch(g, 1);
+  __syncthreads();
+  for (int i = 0; i < steps; ++i) {
+    lay_down(g, i + 1, lds[(i + 1) & 1]);
+    fetch(g, i + 2);
+    multiply(lds[i & 1]);
     __syncthreads();
   }
 
@@ -306,16 +330,13 @@ __global__ __launch_bounds__(256) void checkpoint8_backward_kernel(back_args a) 
       for (int e = 0; e < 16; ++e)
         part[(size_t)(wm + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * BN + wn + j * 32 + (lane & 31)] = acc[i][j][e];
   if (!first_n) return;
+  float *col_sums = reinterpret_cast<float *>(&lds[0]);               // [8][BM]; the last step's readers are past their barrier
 #pragma unroll
-  for (int u = 0; u < UA; ++u) {
-    const int unit = tid + 256 * u;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) col_sums[unit / (BM / 4)][unit % (BM / 4) * 4 + j] = sums[u][j];
-  }
+  for (int j = 0; j < WA; ++j) col_sums[rq * BM + cw * WA + j] = sums[j];
   __syncthreads();
   for (int c = tid; c < BM; c += 256) {
     float s = 0.f;
-    for (int q = 0; q < BK / 4; ++q) s += col_sums[q][c];
+    for (int q = 0; q < 8; ++q) s += col_sums[q * BM + c];
     a.part_b[(size_t)strip * (a.tiles_m * BM) + m0 + c] = s;
   }
 }
@@ -352,7 +373,7 @@ __global__ __launch_bounds__(256) void checkpoint8_reduce_kernel(const float *__
     return;
   }
   const int tile = (int)(at / (BM * BN)), in = (int)(at % (BM * BN)) + threadIdx.x, i = in / BN, j = in % BN;
-  const int o = tile / tiles_n * BM + i % (BM / 4) * 4 + i / (BM / 4), c = tile % tiles_n * BN + j % (BN / 4) * 4 + j / (BN / 4);
+  const int o = tile / tiles_n * BM + i % 32 * (BM / 32) + i / 32, c = tile % tiles_n * BN + j % 32 * (BN / 32) + j / 32;
   if (o < m && c < k) d_w[(size_t)o * k + c] = dg_round<T>(s);
 }
 
@@ -380,36 +401,36 @@ row_grid rows_of(int64_t n, int k) {
   return g;
 }
 
-// Tiles of 128 where that many columns are there; strips so that some 512 workgroups run, of at least 256 rows each.
+// Tiles of 128 columns, or 64 where that leaves fewer of them empty; strips so that some 512 workgroups run, of some 128
+// rows at least each.
+int side_of(int columns) { return (columns + 127) / 128 * 2 > (columns + 63) / 64 ? 64 : 128; }
 struct back_plan {
   int bm, bn, tiles_m, tiles_n, strips;
-  int64_t rows_per_strip;
   size_t part, part_b, bytes;
 };
 back_plan plan_of(int64_t n, int k, int m) {
   back_plan p;
-  p.bm = m > 64 ? 128 : 64;
-  p.bn = k > 64 ? 128 : 64;
+  p.bm = side_of(m);
+  p.bn = m == 1 ? 128 : side_of(k);
   p.tiles_m = (m + p.bm - 1) / p.bm;
   p.tiles_n = (k + p.bn - 1) / p.bn;
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
   int64_t strips = (512 + tiles - 1) / tiles;
-  strips = strips < (n + 255) / 256 ? strips : (n + 255) / 256;
-  p.rows_per_strip = strips ? ((n + strips - 1) / strips + 63) / 64 * 64 : 64;
-  p.strips = (int)((n + p.rows_per_strip - 1) / p.rows_per_strip);
+  strips = strips < (n + 127) / 128 ? strips : (n + 127) / 128;
+  p.strips = (int)strips;
   p.part = 0;
   p.part_b = (size_t)p.strips * tiles * p.bm * p.bn * 4;
   p.bytes = p.part_b + (size_t)p.strips * p.tiles_m * p.bm * 4 + 256;
   return p;
 }
 
-template <typename T, int FMT, bool TANH, int PIECES, int BM, int BN>
+template <typename T, int FMT, bool TANH, int PIECES, int BM, int BN, bool NARROW>
 int back_as(const back_plan &p, const back_args &a, T *d_w, T *d_b, hipStream_t stream) {
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, blocks = (int64_t)(p.strips + 7) / 8 * 8 * tiles;
   if (blocks > 0x7fffffff || tiles * (BM * BN / 64) + p.tiles_m * (BM / 64) > 0x7fffffff)
     return dg_fail(DG_ERR_SIZE, "dg_checkpoint8_backward: a weight of %d x %d is too large", a.m, a.k);
   if (p.strips) {
-    hipLaunchKernelGGL((checkpoint8_backward_kernel<T, FMT, TANH, PIECES, BM, BN>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((checkpoint8_backward_kernel<T, FMT, TANH, PIECES, BM, BN, NARROW>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
     DG_HIP(hipGetLastError());
   }
   hipLaunchKernelGGL((checkpoint8_reduce_kernel<T, BM, BN>), dim3((unsigned)(tiles * (BM * BN / 64) + p.tiles_m * (BM / 64))), dim3(256), 0,
@@ -420,12 +441,13 @@ int back_as(const back_plan &p, const back_args &a, T *d_w, T *d_b, hipStream_t 
 
 template <typename T, int FMT, bool TANH, int PIECES>
 int back_tiles(const back_plan &p, const back_args &a, void *d_w, void *d_b, hipStream_t stream) {
+  if (a.m == 1) return back_as<T, FMT, TANH, PIECES, 64, 128, true>(p, a, (T *)d_w, (T *)d_b, stream);
   if (p.bm == 128) {
-    if (p.bn == 128) return back_as<T, FMT, TANH, PIECES, 128, 128>(p, a, (T *)d_w, (T *)d_b, stream);
-    return back_as<T, FMT, TANH, PIECES, 128, 64>(p, a, (T *)d_w, (T *)d_b, stream);
+    if (p.bn == 128) return back_as<T, FMT, TANH, PIECES, 128, 128, false>(p, a, (T *)d_w, (T *)d_b, stream);
+    return back_as<T, FMT, TANH, PIECES, 128, 64, false>(p, a, (T *)d_w, (T *)d_b, stream);
   }
-  if (p.bn == 128) return back_as<T, FMT, TANH, PIECES, 64, 128>(p, a, (T *)d_w, (T *)d_b, stream);
-  return back_as<T, FMT, TANH, PIECES, 64, 64>(p, a, (T *)d_w, (T *)d_b, stream);
+  if (p.bn == 128) return back_as<T, FMT, TANH, PIECES, 64, 128, false>(p, a, (T *)d_w, (T *)d_b, stream);
+  return back_as<T, FMT, TANH, PIECES, 64, 64, false>(p, a, (T *)d_w, (T *)d_b, stream);
 }
 
 template <typename T, int PLAIN, int WITH_TANH>
@@ -508,11 +530,12 @@ extern "C" int dg_checkpoint8_backward(const void *d_y, int64_t row_stride, int6
     return dg_fail(DG_ERR_ARG, "dg_checkpoint8_backward: NULL argument");
   if (((uintptr_t)x_codes | (uintptr_t)y_codes | (uintptr_t)workspace) & 15)
     return dg_fail(DG_ERR_ARG, "dg_checkpoint8_backward: codes and workspace must be 16-byte aligned");
+  if (row_stride > (1 << 24)) return dg_fail(DG_ERR_SIZE, "dg_checkpoint8_backward: rows of d_y more than 2^24 elements apart");
   const back_plan p = plan_of(n, k, m);
   if (workspace_bytes < p.bytes)
     return dg_fail(DG_ERR_SIZE, "dg_checkpoint8_backward: workspace of %zu bytes, %zu needed", workspace_bytes, p.bytes);
   back_args a = {d_y, row_stride, (const uint8_t *)x_codes, (const uint8_t *)x_scales, (const uint8_t *)y_codes, (const uint8_t *)y_scales,
-                 pitch_of(k), groups_of(k), pitch_of(m), groups_of(m), n, k, m, p.rows_per_strip, p.strips, p.tiles_m, p.tiles_n, d_z,
+                 pitch_of(k), groups_of(k), pitch_of(m), groups_of(m), n, k, m, p.strips, p.tiles_m, p.tiles_n, d_z,
                  (float *)workspace, (float *)((char *)workspace + p.part_b)};
   hipStream_t st = (hipStream_t)stream;
   if (dtype == DG_F32) return back_forms<float, 3, 3>(format, tanh, p, a, d_w, d_b, st);

@@ -244,44 +244,40 @@ __global__ __launch_bounds__(256) void radix_scatter_kernel(key_source s, int64_
 // ---- the same order for short lists, in one launch ---------------------------------------------------------------------
 // An entry's place is the number of entries before it: those of a smaller key, and those of its own key that come earlier.
 // Every workgroup places 32 entries by comparing them with all n (staged in LDS, four keys a read, 32 slices of threads):
-// n^2 comparisons of two instructions each over the whole chip -- 6144 entries: 4.4 us against 25 us for the six launches of
-// two radix passes, which cost about the same at any short length (16384: 17 us).
-constexpr int kRankMax = 16384, kRankTokens = 32, kRankStage = 8192, kRankSlices = 1024 / kRankTokens;
+// n^2 comparisons of two instructions each over the whole chip.  The whole gradient, 64 columns of 60000 rows: 14.1 us at
+// 2048 ids, 18.9 us at 8192 against 23.4 and 28.6 us by the radix passes (launches and their latencies); 33.4 against
+// 31.2 us at 12000, so longer lists go by those.
+constexpr int kRankMax = 8192, kRankTokens = 32, kRankSlices = 1024 / kRankTokens;
 
 __global__ __launch_bounds__(1024) void rank_sort_kernel(key_source s, int n, uint32_t *__restrict__ keys_out,
                                                          uint32_t *__restrict__ pos_out, uint32_t *__restrict__ n_crossing) {
-  __shared__ alignas(16) uint32_t stage[kRankStage];
+  __shared__ alignas(16) uint32_t stage[kRankMax];
   __shared__ uint32_t part[kRankSlices][kRankTokens + 1];
   if (blockIdx.x == 0 && threadIdx.x == 0) *n_crossing = 0;
   const int i0 = blockIdx.x * kRankTokens, t = threadIdx.x % kRankTokens, slice = threadIdx.x / kRankTokens, i = i0 + t;
-  uint32_t own[1], pos[1], rank = 0, r4[4] = {0, 0, 0, 0};
+  constexpr int PER = kRankMax / 1024;
+  uint32_t own[1], pos[1], k[PER], unused[PER], rank = 0, r4[4] = {0, 0, 0, 0};
   load_keys<1>(s, i, 0, n, own, pos);
-  const uint32_t key = own[0];
-  for (int j0 = 0; j0 < n; j0 += kRankStage) {
-    constexpr int PER = kRankStage / 1024;
-    uint32_t k[PER], unused[PER];
-    load_keys<PER>(s, j0 + threadIdx.x, 1024, n, k, unused);
-    __syncthreads();
+  load_keys<PER>(s, threadIdx.x, 1024, n, k, unused);
 #pragma unroll
-    for (int e = 0; e < PER; ++e)                           // (behind the list: smaller than no key)
-      stage[e * 1024 + threadIdx.x] = j0 + e * 1024 + (int)threadIdx.x < n ? k[e] : 0xffffffffu;
-    __syncthreads();
-    // an earlier entry of the same key counts, a later one does not; the workgroup's own entries are taken as later ones
-    const int count = min(kRankStage, n - j0), mid = max(0, min(i0 - j0, count));
-    auto below = [&](int from, int to, uint32_t top) {
+  for (int e = 0; e < PER; ++e)                             // (behind the list: smaller than no key)
+    stage[e * 1024 + threadIdx.x] = e * 1024 + (int)threadIdx.x < n ? k[e] : 0xffffffffu;
+  __syncthreads();
+  const uint32_t key = own[0];
+  auto below = [&](int from, int to, uint32_t top) {
 #pragma unroll 4
-      for (int q = from + slice * 4; q < to; q += 4 * kRankSlices) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(&stage[q]);
-        r4[0] += v.x < top;                                 // (four chains: each step is a compare and an add with carry)
-        r4[1] += v.y < top;
-        r4[2] += v.z < top;
-        r4[3] += v.w < top;
-      }
-    };
-    below(0, mid, key + 1);
-    below(mid, count, key);
-    if (i0 >= j0 && i0 - j0 < kRankStage && slice < t && stage[i0 - j0 + slice] == key) ++rank;   // ... but for these
-  }
+    for (int q = from + slice * 4; q < to; q += 4 * kRankSlices) {
+      const uint4 v = *reinterpret_cast<const uint4 *>(&stage[q]);
+      r4[0] += v.x < top;                                   // (four chains: each step is a compare and an add with carry)
+      r4[1] += v.y < top;
+      r4[2] += v.z < top;
+      r4[3] += v.w < top;
+    }
+  };
+  // an earlier entry of the same key counts, a later one does not; the workgroup's own entries are taken as later ones ...
+  below(0, i0, key + 1);
+  below(i0, n, key);
+  if (slice < t && stage[i0 + slice] == key) ++rank;        // ... but for these
   part[slice][t] = rank + r4[0] + r4[1] + r4[2] + r4[3];
   __syncthreads();
   if (threadIdx.x >= kRankTokens || i >= n) return;

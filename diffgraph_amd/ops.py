@@ -1217,12 +1217,13 @@ def checkpoint8_backward(d_y: torch.Tensor, x: Checkpoint8, y: Optional[Checkpoi
         if y.shape[1] != m or y.format != x.format:
             raise DiffGraphHipError(f"y: expected {m} columns in the format of x ({x.format})")
     lib = _lib.load()
+    src = d_y if n < 2 or d_y.stride(0) <= 1 << 24 else d_y.contiguous()      # (as far apart as the kernel's rows may lie)
     ws_bytes = lib.dg_checkpoint8_backward_workspace(n, k, m)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     d_z = d_y if y is None else torch.empty((n, m), dtype=d_y.dtype, device=dev)
     d_w = torch.empty((m, k), dtype=d_y.dtype, device=dev)
     d_b = torch.empty(m, dtype=d_y.dtype, device=dev)
-    _lib.launch(dev, lib.dg_checkpoint8_backward, "dg_checkpoint8_backward", d_y.data_ptr(), d_y.stride(0), n, m, k, _ELEMENT[d_y.dtype],
+    _lib.launch(dev, lib.dg_checkpoint8_backward, "dg_checkpoint8_backward", src.data_ptr(), src.stride(0) if n > 1 else m, n, m, k, _ELEMENT[d_y.dtype],
                 _FORMATS[x.format], x.codes.data_ptr(), x.scales.data_ptr(), None if y is None else y.codes.data_ptr(),
                 None if y is None else y.scales.data_ptr(), d_z.data_ptr(), d_w.data_ptr(), d_b.data_ptr(), ws.data_ptr(), ws_bytes)
     return d_z, d_w, d_b
