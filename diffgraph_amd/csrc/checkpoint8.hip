@@ -142,20 +142,27 @@ __device__ __forceinline__ uint32_t high_halves(float a, float b) {   // bf16(a)
   return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
 }
 
-// What a thread holds of a step's operands until it lays them down: four rows of WA columns of d_y (and of the codes of
-// y), four rows of WB columns of the codes of x, each row with its group's scale byte.
-template <typename T, int WA, int WB>
+// W neighbouring elements through a buffer descriptor: beyond its end they read as zeros.
+template <int BYTES>
+__device__ __forceinline__ auto load_bytes(__amdgpu_buffer_rsrc_t r, uint32_t at) {
+  if constexpr (BYTES == 16) return __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0);
+  else if constexpr (BYTES == 8) return __builtin_amdgcn_raw_buffer_load_b64(r, at, 0, 0);
+  else if constexpr (BYTES == 4) return __builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0);
+  else if constexpr (BYTES == 2) return __builtin_amdgcn_raw_buffer_load_b16(r, at, 0, 0);
+  else return __builtin_amdgcn_raw_buffer_load_b8(r, at, 0, 0);
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const void *base, int64_t offset, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void *)((const char *)base + offset), 0, bytes, 0x00020000);
+}
+
+// What a thread holds of a block of rows until it lays them down: four rows of WA columns of d_y (and of the codes of y),
+// four rows of WB columns of the codes of x, each row with its group's scale byte.
+template <typename T, int WA>
 struct back_regs {
   dg_vec<T, WA> d[4];
   uint32_t yw[4], ys[4], xw[4], xs[4];
 };
-
-// W neighbouring codes at p (W = 2 or 4; p a multiple of W).
-template <int W>
-__device__ __forceinline__ uint32_t load_codes(const uint8_t *p) {
-  if constexpr (W == 4) return *reinterpret_cast<const uint32_t *>(p);
-  return *reinterpret_cast<const uint16_t *>(p);
-}
 
 // A workgroup sums one strip of rows -- every so many blocks of 32, so that all workgroups together read on through the
 // memory -- for a BM x BN tile of d_w, a block a step: its threads load quads of rows x a few
@@ -163,11 +170,13 @@ __device__ __forceinline__ uint32_t load_codes(const uint8_t *p) {
 // the matrix instruction takes -- transposing in their registers.  A column c of a tile of B sits in slot
 // (c mod W) 32 + c / W, W = B / 32, so that neighbouring lanes write neighbouring slots; results are kept in slot order
 // until the second launch.  Two buffers in LDS and a step on its way in registers: one barrier a step, and the conversion of
-// the next step runs beside the matrix instructions of this one.
+// the next step runs beside the matrix instructions of this one.  A block's rows end with their descriptors: rows behind
+// the last one, and whole blocks behind it, come as zeros, with no branch round a load.
 // NARROW: d_y has one column (a load of two would leave its row).
 template <typename T, int FMT, bool TANH, int PIECES, int BM, int BN, bool NARROW>
 __global__ __launch_bounds__(256) void checkpoint8_backward_kernel(back_args a) {
-  constexpr int BK = 32, WA = BM / 32, WB = BN / 32, WM = BM / 2, WN = BN / 2, TM = WM / 32, TN = WN / 32;
+  constexpr int BK = 32, WA = BM / 32, WB = BN / 32, WM = BM / 2, WN = BN / 2, TM = WM / 32, TN = WN / 32, Z = sizeof(T);
+  constexpr bool RAW = PIECES == 1 && Z == 2 && !TANH;                 // bf16 as it came
   struct buffer {
     u32x4 a[PIECES][BK / 8][BM], b[BK / 8][BN];
   };
@@ -182,10 +191,12 @@ __global__ __launch_bounds__(256) void checkpoint8_backward_kernel(back_args a) 
   const int cw = tid & 31, rq = tid >> 5, steps = (int)(((a.n + BK - 1) / BK - strip + a.strips - 1) / a.strips);
   // columns behind the last one: some other column's values, in rows or columns of the tile that nobody keeps
   const int ca = min(m0 + cw * WA, a.m - 1) / WA * WA, cb = min(n0 + cw * WB, a.k - 1) / WB * WB;
-  const int ga = ca / kGroup, gb = cb / kGroup;
   // the last columns of an odd width are read from further left, and moved into place when they are laid down
   const bool odd = a.m % WA != 0;
   const int from = odd && !NARROW ? min(ca, a.m - WA) : ca, shift = ca - from;
+  const uint32_t r0 = rq * 4, d_pitch = (uint32_t)a.d_stride * Z;
+  const uint32_t at_d = r0 * d_pitch + from * Z, at_y = r0 * a.y_pitch + ca, at_ys = r0 * a.y_groups + ca / kGroup;
+  const uint32_t at_x = r0 * a.x_pitch + cb, at_xs = r0 * a.x_groups + cb / kGroup;
 
   float sums[WA];
 #pragma unroll
@@ -198,52 +209,58 @@ __global__ __launch_bounds__(256) void checkpoint8_backward_kernel(back_args a) 
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
-  auto fetch = [&](back_regs<T, WA, WB> &g, int step) {
-    const int64_t base = ((int64_t)min(step, steps - 1) * a.strips + strip) * BK;      // (no branch: the loads stay countable)
-    const int left = (int)min((int64_t)BK, a.n - base);
-    const T *dy = (const T *)a.d_y + base * a.d_stride;                // (uniform; a lane's part fits 32 bits)
-    const uint8_t *x = a.x + base * a.x_pitch, *xs = a.x_scales + base * a.x_groups;
-    const uint8_t *y = a.y + base * a.y_pitch, *ys = a.y_scales + base * a.y_groups;
+  auto fetch = [&](back_regs<T, WA> &g, int step) {
+    const int64_t base = ((int64_t)step * a.strips + strip) * BK;
+    const int left = (int)max((int64_t)0, min((int64_t)BK, a.n - base));
+    const auto d = rows_at(a.d_y, base * d_pitch, left ? (left - 1) * (int)d_pitch + a.m * Z : 0);
+    const auto x = rows_at(a.x, base * a.x_pitch, left * a.x_pitch), xs = rows_at(a.x_scales, base * a.x_groups, left * a.x_groups);
+    const auto y = rows_at(a.y, base * a.y_pitch, left * a.y_pitch), ys = rows_at(a.y_scales, base * a.y_groups, left * a.y_groups);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const uint32_t r = min(rq * 4 + q, left - 1);                    // (rows behind the strip: cleared when laid down)
-      const T *src = dy + (r * (uint32_t)a.d_stride + from);
-      if constexpr (!NARROW) g.d[q] = dg_load_raw<WA, 2>(src);
-      else g.d[q].v[0] = g.d[q].v[1] = *src;
-      if (TANH) {
-        g.yw[q] = load_codes<WA>(y + (r * (uint32_t)a.y_pitch + ca));
-        g.ys[q] = ys[r * (uint32_t)a.y_groups + ga];
+      if constexpr (!NARROW) {
+        const auto w = load_bytes<WA * Z>(d, at_d + q * d_pitch);
+        __builtin_memcpy(&g.d[q], &w, WA * Z);
+      } else {
+        const auto w = load_bytes<Z>(d, at_d + q * d_pitch);
+        __builtin_memcpy(&g.d[q].v[0], &w, Z);
+        g.d[q].v[1] = g.d[q].v[0];
       }
-      g.xw[q] = load_codes<WB>(x + (r * (uint32_t)a.x_pitch + cb));
-      g.xs[q] = xs[r * (uint32_t)a.x_groups + gb];
+      if (TANH) {
+        g.yw[q] = load_bytes<WA>(y, at_y + q * a.y_pitch);
+        g.ys[q] = load_bytes<1>(ys, at_ys + q * a.y_groups);
+      }
+      g.xw[q] = load_bytes<WB>(x, at_x + q * a.x_pitch);
+      g.xs[q] = load_bytes<1>(xs, at_xs + q * a.x_groups);
     }
   };
 
-  auto lay_down = [&](back_regs<T, WA, WB> &g, int step, buffer &to) {
-    const int64_t base = ((int64_t)step * a.strips + strip) * BK;
-    const int left = step < steps ? (int)min((int64_t)BK, a.n - base) : 0;   // (rows behind the last one: zeros, by selection)
+  auto lay_down = [&](const back_regs<T, WA> &g, int step, buffer &to) {
     float d[4][WA];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int q = 0; q < 4; ++q)
 #pragma unroll
       for (int j = 0; j < WA; ++j) d[q][j] = dg_widen(g.d[q].v[j]);
+    if (odd) {
 #pragma unroll
       for (int by = WA / 2; by; by >>= 1)
 #pragma unroll
-        for (int j = 0; j + by < WA; ++j) {
-          const float here = d[q][j], there = d[q][j + by];
-          d[q][j] = (shift & by) ? there : here;
-        }
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int j = 0; j + by < WA; ++j) {
+            const float here = d[q][j], there = d[q][j + by];
+            d[q][j] = (shift & by) ? there : here;
+          }
     }
     if (TANH) {
+      const int64_t base = ((int64_t)step * a.strips + strip) * BK;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         float y[4];
         decode4<FMT>(g.yw[q], g.ys[q], y);
 #pragma unroll
         for (int j = 0; j < WA; ++j) d[q][j] *= 1.f - y[j] * y[j];
-        if (first_n && rq * 4 + q < left && m0 + cw * WA < a.m) {
-          T *dst = (T *)a.d_z + (base + rq * 4 + q) * a.m + ca;
+        if (first_n && base + r0 + q < a.n && m0 + cw * WA < a.m) {
+          T *dst = (T *)a.d_z + (base + r0 + q) * a.m + ca;
           if (!odd) {
             dg_store_unaligned<WA>(dst, d[q]);
           } else {
@@ -254,28 +271,32 @@ __global__ __launch_bounds__(256) void checkpoint8_backward_kernel(back_args a) 
         }
       }
     }
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const bool in = rq * 4 + q < left;
-#pragma unroll
-      for (int j = 0; j < WA; ++j) d[q][j] = in ? d[q][j] : 0.f;
-      g.xs[q] = in ? g.xs[q] : 0;
-    }
     if (first_n) {
 #pragma unroll
       for (int j = 0; j < WA; ++j) sums[j] += (d[0][j] + d[1][j]) + (d[2][j] + d[3][j]);
     }
+    if (RAW && !odd) {                                                 // two halves of a word, rows paired column by column
 #pragma unroll
-    for (int j = 0; j < WA; ++j) {
-      float v[4] = {d[0][j], d[1][j], d[2][j], d[3][j]};
+      for (int j = 0; j < WA; ++j) {
+        uint32_t w[4];
 #pragma unroll
-      for (int p = 0; p < PIECES; ++p) {
-        u32x2 w;
-        w = {high_halves(v[0], v[1]), high_halves(v[2], v[3])};
-        reinterpret_cast<u32x2 *>(&to.a[p][rq >> 1][j * 32 + cw])[rq & 1] = w;
-        if (p + 1 < PIECES) {
+        for (int q = 0; q < 4; ++q) __builtin_memcpy(&w[q], &g.d[q].v[j & ~1], 4);
+        const uint32_t pick = j & 1 ? 0x07060302u : 0x05040100u;
+        const u32x2 p = {__builtin_amdgcn_perm(w[1], w[0], pick), __builtin_amdgcn_perm(w[3], w[2], pick)};
+        reinterpret_cast<u32x2 *>(&to.a[0][rq >> 1][j * 32 + cw])[rq & 1] = p;
+      }
+    } else {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) v[q] -= __uint_as_float(__float_as_uint(v[q]) & 0xffff0000u);   // (exact)
+      for (int j = 0; j < WA; ++j) {
+        float v[4] = {d[0][j], d[1][j], d[2][j], d[3][j]};
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+          const u32x2 w = {high_halves(v[0], v[1]), high_halves(v[2], v[3])};
+          reinterpret_cast<u32x2 *>(&to.a[p][rq >> 1][j * 32 + cw])[rq & 1] = w;
+          if (p + 1 < PIECES) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] -= __uint_as_float(__float_as_uint(v[q]) & 0xffff0000u);   // (exact)
+          }
         }
       }
     }
@@ -308,16 +329,19 @@ __global__ __launch_bounds__(256) void checkpoint8_backward_kernel(back_args a) 
   };
 
   // Step i is multiplied out of buffer i mod 2 while step i + 1 is laid down in the other and step i + 2 is asked for.
-  // Steps behind the last one are zeros: no branch round a load.
-  back_regs<T, WA, WB> g;
+  back_regs<T, WA> g;
   fetch(g, 0);
   lay_down(g, 0, lds[0]);
   fetch(g, 1);
   __syncthreads();
-  for (int i = 0; i < steps; ++i) {
-    lay_down(g, i + 1, lds[(i + 1) & 1]);
+  for (int i = 0; i < steps; i += 2) {
+    lay_down(g, i + 1, lds[1]);
     fetch(g, i + 2);
-    multiply(lds[i & 1]);
+    multiply(lds[0]);
+    __syncthreads();
+    lay_down(g, i + 2, lds[0]);
+    fetch(g, i + 3);
+    multiply(lds[1]);
     __syncthreads();
   }
 
@@ -341,40 +365,44 @@ __global__ __launch_bounds__(256) void checkpoint8_backward_kernel(back_args a) 
   }
 }
 
-// Adds the strips' parts, 16 strands of every 16th strip each, the strands in order.  A block takes 64 neighbouring
-// values: of a tile (in slot order), or -- the blocks behind them -- of the column sums.
+// Adds the strips' parts: 2^log_strands strands of every so many strips each, the strands in order.  A block takes
+// 1024 >> log_strands neighbouring values: of a tile (in slot order), or -- the blocks behind them -- of the column sums.
 template <typename T, int BM, int BN>
 __global__ __launch_bounds__(256) void checkpoint8_reduce_kernel(const float *__restrict__ part, const float *__restrict__ part_b,
-                                                                 int strips, int tiles_m, int tiles_n, int m, int k,
+                                                                 int strips, int log_strands, int tiles_m, int tiles_n, int m, int k,
                                                                  T *__restrict__ d_w, T *__restrict__ d_b) {
-  __shared__ float strand[16][64];
-  const int tiles = tiles_m * tiles_n, blocks_w = tiles * (BM * BN / 64);
-  const bool bias = (int)blockIdx.x >= blocks_w;
-  const size_t at = bias ? (size_t)(blockIdx.x - blocks_w) * 64 : (size_t)blockIdx.x * 64;
+  __shared__ alignas(16) float strand[1024];
+  const int tiles = tiles_m * tiles_n, per = 1024 >> log_strands, strands = 1 << log_strands, lanes = per / 4;
+  const unsigned blocks_w = (unsigned)tiles * (BM * BN / per);
+  const bool bias = blockIdx.x >= blocks_w;
+  const size_t at = (size_t)(bias ? blockIdx.x - blocks_w : blockIdx.x) * per;
   const size_t step = bias ? (size_t)tiles_m * BM : (size_t)tiles * BM * BN;
-  const float *src = (bias ? part_b : part) + at;
-  const int g = threadIdx.x >> 4, l = threadIdx.x & 15;
+  const int g = threadIdx.x / lanes, l = threadIdx.x % lanes;
+  const float *src = (bias ? part_b : part) + at + 4 * l;
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int s = g; s < strips; s += 16) {
-    float f[4];
-    dg_load<4>(src + s * step + 4 * l, f);
+  if (at + 4 * l < step) {
+#pragma unroll 4
+    for (int s = g; s < strips; s += strands) {
+      float f[4];
+      dg_load<4>(src + s * step, f);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] += f[e];
+      for (int e = 0; e < 4; ++e) acc[e] += f[e];
+    }
   }
 #pragma unroll
-  for (int e = 0; e < 4; ++e) strand[g][4 * l + e] = acc[e];
+  for (int e = 0; e < 4; ++e) strand[g * per + 4 * l + e] = acc[e];
   __syncthreads();
-  if (threadIdx.x >= 64) return;
-  float s = strand[0][threadIdx.x];
-  for (int q = 1; q < 16; ++q) s += strand[q][threadIdx.x];
-  if (bias) {
-    const size_t o = at + threadIdx.x;
-    if (o < (size_t)m) d_b[o] = dg_round<T>(s);
-    return;
+  for (int v = threadIdx.x; v < per; v += 256) {
+    float s = strand[v];
+    for (int q = 1; q < strands; ++q) s += strand[q * per + v];
+    if (bias) {
+      if (at + v < (size_t)m) d_b[at + v] = dg_round<T>(s);
+      continue;
+    }
+    const int tile = (int)(at / (BM * BN)), in = (int)(at % (BM * BN)) + v, i = in / BN, j = in % BN;
+    const int o = tile / tiles_n * BM + i % 32 * (BM / 32) + i / 32, c = tile % tiles_n * BN + j % 32 * (BN / 32) + j / 32;
+    if (o < m && c < k) d_w[(size_t)o * k + c] = dg_round<T>(s);
   }
-  const int tile = (int)(at / (BM * BN)), in = (int)(at % (BM * BN)) + threadIdx.x, i = in / BN, j = in % BN;
-  const int o = tile / tiles_n * BM + i % 32 * (BM / 32) + i / 32, c = tile % tiles_n * BN + j % 32 * (BN / 32) + j / 32;
-  if (o < m && c < k) d_w[(size_t)o * k + c] = dg_round<T>(s);
 }
 
 // ---- host side --------------------------------------------------------------------------------------------------
@@ -427,14 +455,17 @@ back_plan plan_of(int64_t n, int k, int m) {
 template <typename T, int FMT, bool TANH, int PIECES, int BM, int BN, bool NARROW>
 int back_as(const back_plan &p, const back_args &a, T *d_w, T *d_b, hipStream_t stream) {
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, blocks = (int64_t)(p.strips + 7) / 8 * 8 * tiles;
-  if (blocks > 0x7fffffff || tiles * (BM * BN / 64) + p.tiles_m * (BM / 64) > 0x7fffffff)
-    return dg_fail(DG_ERR_SIZE, "dg_checkpoint8_backward: a weight of %d x %d is too large", a.m, a.k);
+  int log_strands = 0;
+  while (log_strands < 6 && (2 << log_strands) <= p.strips) ++log_strands;
+  const int per = 1024 >> log_strands;
+  const int64_t sums = tiles * (BM * BN / per) + ((int64_t)p.tiles_m * BM + per - 1) / per;
+  if (blocks > 0x7fffffff || sums > 0x7fffffff) return dg_fail(DG_ERR_SIZE, "dg_checkpoint8_backward: a weight of %d x %d is too large", a.m, a.k);
   if (p.strips) {
     hipLaunchKernelGGL((checkpoint8_backward_kernel<T, FMT, TANH, PIECES, BM, BN, NARROW>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
     DG_HIP(hipGetLastError());
   }
-  hipLaunchKernelGGL((checkpoint8_reduce_kernel<T, BM, BN>), dim3((unsigned)(tiles * (BM * BN / 64) + p.tiles_m * (BM / 64))), dim3(256), 0,
-                     stream, a.part, a.part_b, p.strips, p.tiles_m, p.tiles_n, a.m, a.k, d_w, d_b);
+  hipLaunchKernelGGL((checkpoint8_reduce_kernel<T, BM, BN>), dim3((unsigned)sums), dim3(256), 0, stream, a.part, a.part_b, p.strips,
+                     log_strands, p.tiles_m, p.tiles_n, a.m, a.k, d_w, d_b);
   DG_HIP(hipGetLastError());
   return 0;
 }
@@ -524,13 +555,13 @@ extern "C" int dg_checkpoint8_backward(const void *d_y, int64_t row_stride, int6
   if (const int rc = check_sizes("dg_checkpoint8_backward", n, k, format)) return rc;
   if (const int rc = check_sizes("dg_checkpoint8_backward", n, m, format)) return rc;
   if (!type_size(dtype)) return dg_fail(DG_ERR_ARG, "dg_checkpoint8_backward: unknown element type %d", dtype);
-  if (row_stride < 0) return dg_fail(DG_ERR_ARG, "dg_checkpoint8_backward: negative row stride");
   const bool tanh = y_codes != nullptr;
   if (!d_w || !d_b || !workspace || (n && (!d_y || !x_codes || !x_scales || (tanh && (!y_scales || !d_z)))))
     return dg_fail(DG_ERR_ARG, "dg_checkpoint8_backward: NULL argument");
   if (((uintptr_t)x_codes | (uintptr_t)y_codes | (uintptr_t)workspace) & 15)
     return dg_fail(DG_ERR_ARG, "dg_checkpoint8_backward: codes and workspace must be 16-byte aligned");
   if (row_stride > (1 << 24)) return dg_fail(DG_ERR_SIZE, "dg_checkpoint8_backward: rows of d_y more than 2^24 elements apart");
+  if (row_stride < m) return dg_fail(DG_ERR_ARG, "dg_checkpoint8_backward: rows of d_y overlap");
   const back_plan p = plan_of(n, k, m);
   if (workspace_bytes < p.bytes)
     return dg_fail(DG_ERR_SIZE, "dg_checkpoint8_backward: workspace of %zu bytes, %zu needed", workspace_bytes, p.bytes);

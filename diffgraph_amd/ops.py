@@ -1217,7 +1217,7 @@ def checkpoint8_backward(d_y: torch.Tensor, x: Checkpoint8, y: Optional[Checkpoi
         if y.shape[1] != m or y.format != x.format:
             raise DiffGraphHipError(f"y: expected {m} columns in the format of x ({x.format})")
     lib = _lib.load()
-    src = d_y if n < 2 or d_y.stride(0) <= 1 << 24 else d_y.contiguous()      # (as far apart as the kernel's rows may lie)
+    src = d_y if n < 2 or m <= d_y.stride(0) <= 1 << 24 else d_y.contiguous()      # (as the kernel's rows may lie)
     ws_bytes = lib.dg_checkpoint8_backward_workspace(n, k, m)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     d_z = d_y if y is None else torch.empty((n, m), dtype=d_y.dtype, device=dev)

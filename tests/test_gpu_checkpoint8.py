@@ -190,6 +190,18 @@ def test_backward_of_real_numbers(n, m, k, dtype, tanh, fmt):
 
 
 @gpu
+def test_rows_of_the_gradient_far_apart_or_the_same():
+    xk = ops.checkpoint8(torch.randn(5, 40, device=DEV))
+    far = torch.zeros(5, (1 << 24) + 3, device=DEV)[:, :6]
+    far.normal_()
+    same = torch.randn(1, 6, device=DEV).expand(5, 6)
+    for d in (far, same):
+        _, d_w, d_b = ops.checkpoint8_backward(d, xk)
+        _, w, b = ops.checkpoint8_backward(d.clone(memory_format=torch.contiguous_format), xk)
+        assert torch.equal(d_w, w) and torch.equal(d_b, b)
+
+
+@gpu
 def test_no_rows_give_zeros():
     for tanh in (False, True):
         xk, yk = ops.checkpoint8(torch.zeros(0, 40, device=DEV)), ops.checkpoint8(torch.zeros(0, 9, device=DEV))
@@ -254,10 +266,11 @@ def test_c_entry_refuses_bad_arguments():
     need = lib.dg_checkpoint8_backward_workspace(100, 8, 8)
     back = lambda **k: lib.dg_checkpoint8_backward(*{**dict(d_y=p, stride=8, n=100, m=8, k=8, dtype=0, fmt=0, xc=p, xs=p, yc=p, ys=p, dz=p,  # noqa: E731
                                                             dw=p, db=p, ws=p, bytes=need, stream=None), **k}.values())
-    for bad, text in ((dict(fmt=2), b"format"), (dict(dtype=3), b"type"), (dict(m=0), b"sizes"), (dict(n=-1), b"sizes"), (dict(stride=-1), b"stride"),
+    for bad, text in ((dict(fmt=2), b"format"), (dict(dtype=3), b"type"), (dict(m=0), b"sizes"), (dict(n=-1), b"sizes"), (dict(stride=7), b"overlap"),
                       (dict(xc=None), b"NULL"), (dict(ys=None), b"NULL"), (dict(dz=None), b"NULL"), (dict(dw=None), b"NULL"),
                       (dict(xc=p + 4), b"aligned"), (dict(ws=p + 4), b"aligned")):
         assert back(**bad) == -1 and text in lib.dg_last_error(), bad
+    assert back(stride=(1 << 24) + 1) == -3 and b"apart" in lib.dg_last_error()
     assert back(bytes=need - 1) == -3 and b"workspace" in lib.dg_last_error()
 
 
