@@ -189,12 +189,11 @@ SIGNATURES = {
     "dg_adam_multi": (C.c_int, [C.POINTER(C.c_void_p)] * 4 + [C.POINTER(C.c_int64), C.c_int32, C.c_void_p] + [C.c_float] * 5
                       + [C.c_void_p]),
     "dg_clear": (C.c_int, [C.c_void_p, C.c_size_t, C.c_void_p]),
-    "dg_checkpoint8_pitch": (C.c_int32, [C.c_int32]),
-    "dg_checkpoint8_groups": (C.c_int32, [C.c_int32]),
-    "dg_checkpoint8": (C.c_int, [C.c_void_p, C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p]),
-    "dg_checkpoint8_values": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p]),
+    "dg_checkpoint8_bytes": (C.c_size_t, [C.c_int64, C.c_int32]),
+    "dg_checkpoint8": (C.c_int, [C.c_void_p, C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p]),
+    "dg_checkpoint8_values": (C.c_int, [C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p]),
     "dg_checkpoint8_backward_workspace": (C.c_size_t, [C.c_int64, C.c_int32, C.c_int32]),
-    "dg_checkpoint8_backward": (C.c_int, [C.c_void_p, C.c_int64, C.c_int64] + [C.c_int32] * 4 + [C.c_void_p] * 8 + [C.c_size_t, C.c_void_p]),
+    "dg_checkpoint8_backward": (C.c_int, [C.c_void_p, C.c_int64, C.c_int64] + [C.c_int32] * 4 + [C.c_void_p] * 6 + [C.c_size_t, C.c_void_p]),
     "dg_adjust_scores": (C.c_int, [C.POINTER(ScoreTask), C.c_void_p]),
     "dg_embedding_lookup": (C.c_int, [C.c_void_p, C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_int32, C.c_int64,
                                       C.c_float, C.c_void_p, C.c_void_p]),

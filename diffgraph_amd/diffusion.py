@@ -56,30 +56,28 @@ class _Dense8Fn(torch.autograd.Function):
     layer behind it keeps nothing of its own.  The gradient of the input is exact; d_w and tanh' are formed from the codes."""
 
     @staticmethod
-    def forward(ctx, x, codes, scales, w, b, fmt, tanh):
+    def forward(ctx, x, kept, w, b, fmt, tanh):
         x, w = x.contiguous(), w.contiguous()
-        xk = ops.checkpoint8(x, fmt) if codes is None else ops.Checkpoint8(codes, scales, tuple(x.shape), fmt)
-        y = ops.linear_fwd(x, w, b)
-        yk = None
+        if kept is None:
+            kept = ops.checkpoint8(x, fmt).data
+        y, y_kept = ops.linear_fwd(x, w, b), None
         if tanh:
             y = torch.tanh(y)
-            yk = ops.checkpoint8(y, fmt)
-        ctx.save_for_backward(w, xk.codes, xk.scales, *((yk.codes, yk.scales) if tanh else ()))
-        ctx.aux = (fmt, xk.shape, tuple(y.shape))
-        if not tanh:
-            return y, None, None
-        ctx.mark_non_differentiable(yk.codes, yk.scales)
-        return y, yk.codes, yk.scales
+            y_kept = ops.checkpoint8(y, fmt).data
+            ctx.mark_non_differentiable(y_kept)
+        ctx.save_for_backward(w, kept, *((y_kept,) if tanh else ()))
+        ctx.aux = (fmt, tuple(x.shape), tuple(y.shape))
+        return y, y_kept
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, dy, _codes, _scales):
-        w, xc, xs, *y = ctx.saved_tensors
+    def backward(ctx, dy, _kept):
+        w, kept, *y = ctx.saved_tensors
         fmt, x_shape, y_shape = ctx.aux
-        yk = ops.Checkpoint8(*y, y_shape, fmt) if y else None
-        d_z, d_w, d_b = ops.checkpoint8_backward(dy.contiguous(), ops.Checkpoint8(xc, xs, x_shape, fmt), yk)
+        y = ops.Checkpoint8(y[0], y_shape, fmt) if y else None
+        d_z, d_w, d_b = ops.checkpoint8_backward(dy.contiguous(), ops.Checkpoint8(kept, x_shape, fmt), y)
         d_x = ops.linear_fwd(d_z, w.t().contiguous(), None) if ctx.needs_input_grad[0] else None
-        return d_x, None, None, d_w, d_b, None, None
+        return d_x, None, d_w, d_b, None, None
 
 
 class Denoise(nn.Module):
@@ -172,11 +170,11 @@ class Denoise(nn.Module):
                 x = self.drop(x)
         h = torch.cat([x, emb], dim=-1)
         if self.act_ckpt is not None and torch.is_grad_enabled():
-            codes = scales = None
+            kept = None
             dense = [(layer, True) for layer in self.in_layers]
             dense += [(layer, i != len(self.out_layers) - 1) for i, layer in enumerate(self.out_layers)]
             for layer, tanh in dense:
-                h, codes, scales = _Dense8Fn.apply(h, codes, scales, layer.weight, layer.bias, self.act_ckpt, tanh)
+                h, kept = _Dense8Fn.apply(h, kept, layer.weight, layer.bias, self.act_ckpt, tanh)
             return h if wide == self.width else torch.nn.functional.pad(h, (0, wide - self.width))
         for layer in self.in_layers:
             h = torch.tanh(_LinearFn.apply(h, layer.weight, layer.bias))

@@ -1159,10 +1159,9 @@ _FORMATS = {"int8": _lib.DG_INT8, "e4m3": _lib.DG_E4M3}
 
 @dataclass
 class Checkpoint8:
-    """What is kept of an activation [n, k]: one code byte per element and one scale byte per 32 columns of a row
-    (checkpoint8).  A group that held an infinity or a NaN stands for NaN as a whole."""
-    codes: torch.Tensor         # uint8 [n, k rounded up to 16]
-    scales: torch.Tensor        # uint8 [n, ceil(k / 32)]: exponent + 127, 255 = NaN
+    """What is kept of an activation [n, k] (checkpoint8): a code byte per element and a scale byte per 32 columns of a row,
+    in one buffer.  A group that held an infinity or a NaN stands for NaN as a whole."""
+    data: torch.Tensor          # uint8, dg_checkpoint8_bytes(n, k) of them
     shape: tuple
     format: str
 
@@ -1171,21 +1170,24 @@ class Checkpoint8:
         if dtype not in _ELEMENT:
             raise DiffGraphHipError(f"values: float32, bfloat16 or float16, not {dtype}")
         n, k = self.shape
-        dev = self.codes.device
+        dev = self.data.device
+        self._check("values", n, dev)
         out = torch.empty((n, k), dtype=dtype, device=dev)
-        _lib.launch(dev, _lib.load().dg_checkpoint8_values, "dg_checkpoint8_values", self.codes.data_ptr(), self.scales.data_ptr(), n, k,
-                    _FORMATS[self.format], _ELEMENT[dtype], out.data_ptr())
+        _lib.launch(dev, _lib.load().dg_checkpoint8_values, "dg_checkpoint8_values", self.data.data_ptr(), n, k, _FORMATS[self.format],
+                    _ELEMENT[dtype], out.data_ptr())
         return out
 
-    def check(self, name: str, n: int, device) -> None:
-        if not isinstance(self, Checkpoint8):
-            raise DiffGraphHipError(f"{name}: expected what checkpoint8 returns")
-        k = self.shape[1]
-        for t, w in ((self.codes, (k + 15) // 16 * 16), (self.scales, (k + 31) // 32)):
-            if t.dtype != torch.uint8 or t.device != device or tuple(t.shape) != (self.shape[0], w) or not t.is_contiguous():
-                raise DiffGraphHipError(f"{name}: its codes and scales are not checkpoint8's, or on another device than {device}")
+    def _check(self, name: str, n: int, device) -> None:
+        d, k = self.data, self.shape[1]
+        if not d.is_cuda or d.device != device or d.dtype != torch.uint8 or d.numel() != _kept_bytes(self.shape[0], k) or not d.is_contiguous() \
+                or self.format not in _FORMATS:
+            raise DiffGraphHipError(f"{name}: not what checkpoint8 keeps, or on another device")
         if self.shape[0] != n:
             raise DiffGraphHipError(f"{name}: kept of {self.shape[0]} rows, the gradient has {n}")
+
+
+def _kept_bytes(n: int, k: int) -> int:
+    return (n + 3) // 4 * 4 * ((k + 15) // 16 * 16 + (k + 31) // 32)
 
 
 def checkpoint8(x: torch.Tensor, format: str = "int8") -> Checkpoint8:
@@ -1196,11 +1198,10 @@ def checkpoint8(x: torch.Tensor, format: str = "int8") -> Checkpoint8:
         raise DiffGraphHipError(f"format: 'int8' or 'e4m3', got {format!r}")
     n, k = x.shape
     dev = x.device
-    codes = torch.empty((n, (k + 15) // 16 * 16), dtype=torch.uint8, device=dev)
-    scales = torch.empty((n, (k + 31) // 32), dtype=torch.uint8, device=dev)
+    data = torch.empty(_kept_bytes(n, k), dtype=torch.uint8, device=dev)
     _lib.launch(dev, _lib.load().dg_checkpoint8, "dg_checkpoint8", x.data_ptr(), x.stride(0), n, k, _ELEMENT[x.dtype], _FORMATS[format],
-                codes.data_ptr(), scales.data_ptr())
-    return Checkpoint8(codes, scales, (n, k), format)
+                data.data_ptr())
+    return Checkpoint8(data, (n, k), format)
 
 
 def checkpoint8_backward(d_y: torch.Tensor, x: Checkpoint8, y: Optional[Checkpoint8] = None):
@@ -1210,10 +1211,12 @@ def checkpoint8_backward(d_y: torch.Tensor, x: Checkpoint8, y: Optional[Checkpoi
     _rows(d_y, "d_y")
     n, m = d_y.shape
     dev = d_y.device
-    Checkpoint8.check(x, "x", n, dev)
+    if not isinstance(x, Checkpoint8) or not (y is None or isinstance(y, Checkpoint8)):
+        raise DiffGraphHipError("x, y: expected what checkpoint8 returns")
+    x._check("x", n, dev)
     k = x.shape[1]
     if y is not None:
-        Checkpoint8.check(y, "y", n, dev)
+        y._check("y", n, dev)
         if y.shape[1] != m or y.format != x.format:
             raise DiffGraphHipError(f"y: expected {m} columns in the format of x ({x.format})")
     lib = _lib.load()
@@ -1223,7 +1226,7 @@ def checkpoint8_backward(d_y: torch.Tensor, x: Checkpoint8, y: Optional[Checkpoi
     d_z = d_y if y is None else torch.empty((n, m), dtype=d_y.dtype, device=dev)
     d_w = torch.empty((m, k), dtype=d_y.dtype, device=dev)
     d_b = torch.empty(m, dtype=d_y.dtype, device=dev)
-    _lib.launch(dev, lib.dg_checkpoint8_backward, "dg_checkpoint8_backward", src.data_ptr(), src.stride(0) if n > 1 else m, n, m, k, _ELEMENT[d_y.dtype],
-                _FORMATS[x.format], x.codes.data_ptr(), x.scales.data_ptr(), None if y is None else y.codes.data_ptr(),
-                None if y is None else y.scales.data_ptr(), d_z.data_ptr(), d_w.data_ptr(), d_b.data_ptr(), ws.data_ptr(), ws_bytes)
+    _lib.launch(dev, lib.dg_checkpoint8_backward, "dg_checkpoint8_backward", src.data_ptr(), src.stride(0) if n > 1 else m, n, m, k,
+                _ELEMENT[d_y.dtype], _FORMATS[x.format], x.data.data_ptr(), None if y is None else y.data.data_ptr(), d_z.data_ptr(),
+                d_w.data_ptr(), d_b.data_ptr(), ws.data_ptr(), ws_bytes)
     return d_z, d_w, d_b

@@ -754,34 +754,33 @@ int dg_adjust_scores(const dg_score_task *task, void *stream);
 /* ------------------------------------------------------------------------------------
  * Activation checkpoints in 8 bits and the backward pass of a dense layer out of them (the denoisers' nn.Linear and tanh,
  * DiffGraph-Rec/Model.py:226-233).
- *   dg_checkpoint8           codes[n][pitch] and scales[n][groups] of x [n][k]: per group of 32 columns of a row the smallest
- *                            power of two 2^s, s >= -110, with (largest magnitude) <= Q 2^s, Q = 127 (DG_INT8) or 448
- *                            (DG_E4M3); code = x / 2^s to the nearest code, ties to even.  scales holds s + 127, 255 for a
- *                            group with an infinity or a NaN in it, which stands for NaN as a whole.  Columns k .. pitch - 1
- *                            are zero codes.  pitch = dg_checkpoint8_pitch(k), groups = dg_checkpoint8_groups(k)
+ *   dg_checkpoint8           keeps x [n][k] in dg_checkpoint8_bytes(n, k) bytes: a code byte per element and, per group of
+ *                            32 columns of a row, a scale byte s + 127 for the smallest power of two 2^s, s >= -110, with
+ *                            (largest magnitude) <= Q 2^s, Q = 127 (DG_INT8) or 448 (DG_E4M3); code = x / 2^s to the
+ *                            nearest code, ties to even.  A group with an infinity or a NaN in it has scale byte 255 and
+ *                            stands for NaN as a whole.  Layout: code (r, c) at (r / 4) 4 P + 4 c + r % 4, P = k rounded
+ *                            up to 16; behind the ceil(n / 4) 4 P bytes of the codes the scale of (r, g) at
+ *                            (r / 4) 4 G + 4 g + r % 4, G = ceil(k / 32); zeros where there is no row or column
  *   dg_checkpoint8_values    what they stand for, out [n][k] contiguous
- *   dg_checkpoint8_backward  of y = x . w^T + b (y_codes NULL) or y = tanh(x . w^T + b), from d_y [n][m], the codes of
- *                            x [n][k] and, with tanh, of y [n][m]:
+ *   dg_checkpoint8_backward  of y = x . w^T + b (y_kept NULL) or y = tanh(x . w^T + b), from d_y [n][m], what was kept of
+ *                            x [n][k] and, with tanh, of y [n][m] (both in `format`):
  *                              d_z = d_y (1 - y y) (written with tanh only), d_w[m][k] = d_z^T . x, d_b[m] = column sums
  *                            in fp32 over strips of rows added in strip order, every output rounded once to dtype.  An
  *                            infinity in d_y gives NaN in its column of d_w
- * dtype (x, out, d_y, d_z, d_w, d_b): DG_F32 / DG_BF16 / DG_F16; row_stride: elements between the rows of x / d_y.
- * codes and workspace: 16-byte aligned.  workspace: DEVICE, dg_checkpoint8_backward_workspace bytes, contents irrelevant;
- * calls that may run at the same time need one each.
+ * dtype (x, out, d_y, d_z, d_w, d_b): DG_F32 / DG_BF16 / DG_F16; row_stride: elements between the rows of x / d_y (of d_y:
+ * m to 2^24).  Kept bytes and workspace: DEVICE, 16-byte aligned.  workspace: dg_checkpoint8_backward_workspace bytes,
+ * contents irrelevant; calls that may run at the same time need one each.
  * ---------------------------------------------------------------------------------- */
 #define DG_INT8 0
 #define DG_E4M3 1
-int32_t dg_checkpoint8_pitch(int32_t k);
-int32_t dg_checkpoint8_groups(int32_t k);
-int dg_checkpoint8(const void *x, int64_t row_stride, int64_t n, int32_t k, int32_t dtype, int32_t format, void *codes,
-                   void *scales, void *stream);
-int dg_checkpoint8_values(const void *codes, const void *scales, int64_t n, int32_t k, int32_t format, int32_t dtype,
-                          void *out, void *stream);
+size_t dg_checkpoint8_bytes(int64_t n, int32_t k);
+int dg_checkpoint8(const void *x, int64_t row_stride, int64_t n, int32_t k, int32_t dtype, int32_t format, void *kept,
+                   void *stream);
+int dg_checkpoint8_values(const void *kept, int64_t n, int32_t k, int32_t format, int32_t dtype, void *out, void *stream);
 size_t dg_checkpoint8_backward_workspace(int64_t n, int32_t k, int32_t m);
 int dg_checkpoint8_backward(const void *d_y, int64_t row_stride, int64_t n, int32_t m, int32_t k, int32_t dtype,
-                            int32_t format, const void *x_codes, const void *x_scales, const void *y_codes,
-                            const void *y_scales, void *d_z, void *d_w, void *d_b, void *workspace,
-                            size_t workspace_bytes, void *stream);
+                            int32_t format, const void *x_kept, const void *y_kept, void *d_z, void *d_w, void *d_b,
+                            void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

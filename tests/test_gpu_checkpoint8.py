@@ -54,17 +54,19 @@ def check_kept(x, fmt):
     ck = ops.checkpoint8(x, fmt)
     n, k = x.shape
     want, scale = want_values(x, fmt)
-    assert ck.shape == (n, k) and ck.codes.shape == (n, (k + 15) // 16 * 16) and ck.scales.shape == (n, (k + 31) // 32)
-    byte = ck.scales.cpu().double()
+    pitch, groups, quads = (k + 15) // 16 * 16, (k + 31) // 32, (n + 3) // 4
+    assert ck.shape == (n, k) and ck.data.numel() == _lib.load().dg_checkpoint8_bytes(n, k) == 4 * quads * (pitch + groups)
+    codes = ck.data[: 4 * quads * pitch].view(quads, pitch, 4).permute(0, 2, 1).reshape(4 * quads, pitch).cpu()
+    byte = ck.data[4 * quads * pitch:].view(quads, groups, 4).permute(0, 2, 1).reshape(4 * quads, groups)[:n].cpu().double()
     assert torch.equal(torch.where(byte == 255, torch.full_like(byte, math.nan), 2.0 ** (byte - 127)).nan_to_num(-1), scale.nan_to_num(-1))
-    assert not bool(ck.codes[:, k:].any())
+    assert not bool(codes[:, k:].any()) and not bool(codes[n:].any())
     for t in TYPES:
         got = ck.values(t).cpu()
         assert got.dtype == t and torch.equal(got.double().nan_to_num(7e37), want.to(torch.float32).to(t).double().nan_to_num(7e37))
     return ck, want
 
 
-SIZES = [(1, 1), (1, 7), (3, 8), (1, 16), (5, 31), (64, 32), (7, 33), (129, 72), (33, 100), (4, 333), (17, 1000), (3, 2050), (300, 64)]
+SIZES = [(1, 1), (1, 7), (2, 3), (3, 8), (1, 16), (5, 31), (64, 32), (7, 33), (129, 72), (33, 100), (4, 333), (17, 1000), (3, 2050), (300, 64)]
 
 
 @gpu
@@ -253,22 +255,22 @@ def test_on_another_stream_and_in_a_graph():
 # ---- refusals (no GPU needed) ---------------------------------------------------------------------------------------
 def test_c_entry_refuses_bad_arguments():
     lib, p = _lib.load(), 1 << 20
-    assert lib.dg_checkpoint8_pitch(33) == 48 and lib.dg_checkpoint8_groups(33) == 2 and lib.dg_checkpoint8_pitch(0) == 0
-    assert lib.dg_checkpoint8(p, 8, 2, 8, 0, 5, p, p, None) == -1 and b"format" in lib.dg_last_error()
-    assert lib.dg_checkpoint8(p, 8, 2, 8, 9, 0, p, p, None) == -1 and b"type" in lib.dg_last_error()
-    assert lib.dg_checkpoint8(p, 8, 2, 0, 0, 0, p, p, None) == -1
-    assert lib.dg_checkpoint8(p, -8, 2, 8, 0, 0, p, p, None) == -1
-    assert lib.dg_checkpoint8(p, 8, 2, 8, 0, 0, p + 8, p, None) == -1 and b"aligned" in lib.dg_last_error()
-    assert lib.dg_checkpoint8(None, 8, 2, 8, 0, 0, p, p, None) == -1
-    assert lib.dg_checkpoint8(None, 8, 0, 8, 0, 0, None, None, None) == 0
-    assert lib.dg_checkpoint8(p, 8, 1 << 31, 8, 0, 0, p, p, None) == -3
-    assert lib.dg_checkpoint8_values(p, p, 2, 8, 0, 9, p, None) == -1 and lib.dg_checkpoint8_values(p, None, 2, 8, 0, 0, p, None) == -1
+    assert lib.dg_checkpoint8_bytes(5, 33) == 8 * (48 + 2) and lib.dg_checkpoint8_bytes(5, 0) == 0 and lib.dg_checkpoint8_bytes(-1, 4) == 0
+    assert lib.dg_checkpoint8(p, 8, 2, 8, 0, 5, p, None) == -1 and b"format" in lib.dg_last_error()
+    assert lib.dg_checkpoint8(p, 8, 2, 8, 9, 0, p, None) == -1 and b"type" in lib.dg_last_error()
+    assert lib.dg_checkpoint8(p, 8, 2, 0, 0, 0, p, None) == -1
+    assert lib.dg_checkpoint8(p, -8, 2, 8, 0, 0, p, None) == -1
+    assert lib.dg_checkpoint8(p, 8, 2, 8, 0, 0, p + 8, None) == -1 and b"aligned" in lib.dg_last_error()
+    assert lib.dg_checkpoint8(None, 8, 2, 8, 0, 0, p, None) == -1
+    assert lib.dg_checkpoint8(None, 8, 0, 8, 0, 0, None, None) == 0
+    assert lib.dg_checkpoint8(p, 8, 1 << 31, 8, 0, 0, p, None) == -3
+    assert lib.dg_checkpoint8_values(p, 2, 8, 0, 9, p, None) == -1 and lib.dg_checkpoint8_values(None, 2, 8, 0, 0, p, None) == -1
     need = lib.dg_checkpoint8_backward_workspace(100, 8, 8)
-    back = lambda **k: lib.dg_checkpoint8_backward(*{**dict(d_y=p, stride=8, n=100, m=8, k=8, dtype=0, fmt=0, xc=p, xs=p, yc=p, ys=p, dz=p,  # noqa: E731
+    back = lambda **k: lib.dg_checkpoint8_backward(*{**dict(d_y=p, stride=8, n=100, m=8, k=8, dtype=0, fmt=0, xk=p, yk=p, dz=p,  # noqa: E731
                                                             dw=p, db=p, ws=p, bytes=need, stream=None), **k}.values())
     for bad, text in ((dict(fmt=2), b"format"), (dict(dtype=3), b"type"), (dict(m=0), b"sizes"), (dict(n=-1), b"sizes"), (dict(stride=7), b"overlap"),
-                      (dict(xc=None), b"NULL"), (dict(ys=None), b"NULL"), (dict(dz=None), b"NULL"), (dict(dw=None), b"NULL"),
-                      (dict(xc=p + 4), b"aligned"), (dict(ws=p + 4), b"aligned")):
+                      (dict(xk=None), b"NULL"), (dict(dz=None), b"NULL"), (dict(dw=None), b"NULL"),
+                      (dict(xk=p + 4), b"aligned"), (dict(yk=p + 8), b"aligned"), (dict(ws=p + 4), b"aligned")):
         assert back(**bad) == -1 and text in lib.dg_last_error(), bad
     assert back(stride=(1 << 24) + 1) == -3 and b"apart" in lib.dg_last_error()
     assert back(bytes=need - 1) == -3 and b"workspace" in lib.dg_last_error()
@@ -290,6 +292,7 @@ def test_wrong_arguments_are_refused():
                        (lambda: ops.checkpoint8_backward(d, x), "checkpoint8 returns"), (lambda: ops.checkpoint8_backward(d[:5], xk), "rows"),
                        (lambda: ops.checkpoint8_backward(d, xk, xk), "columns"),
                        (lambda: ops.checkpoint8_backward(d, xk, ops.checkpoint8(d, "e4m3")), "format"),
-                       (lambda: ops.checkpoint8_backward(d, ops.Checkpoint8(xk.codes[:, :40], xk.scales, (6, 40), "int8")), "codes")):
+                       (lambda: ops.checkpoint8_backward(d, ops.Checkpoint8(xk.data[:-1], (6, 40), "int8")), "keeps"),
+                       (lambda: ops.Checkpoint8(xk.data, (6, 49), "int8").values(), "keeps")):
         with pytest.raises(DiffGraphHipError, match=what):
             call()
