@@ -199,7 +199,7 @@ struct back_regs {
 // columns, form d_z, cut it, and lay both operands down in LDS with eight rows of a column in 16 bytes -- what a lane of
 // the matrix instruction takes -- transposing in their registers.  A column c of a tile of B sits in slot
 // (c mod W) 32 + c / W, W = B / 32, so that neighbouring lanes write neighbouring slots; results are kept in slot order
-// until the second launch.  Two buffers in LDS and a step on its way in registers: one barrier a step, and the conversion of
+// until the second launch.  Two buffers in LDS and two steps on their way in registers: one barrier a step, and the conversion of
 // the next step runs beside the matrix instructions of this one.  A block's rows end with their descriptors: rows behind
 // the last one, and whole blocks behind it, come as zeros, with no branch round a load.
 // NARROW: d_y has one column (a load of two would leave its row).
@@ -212,13 +212,15 @@ __global__ __launch_bounds__(256) void checkpoint8_backward_kernel(back_args a) 
   };
   __shared__ buffer lds[2];
   const int tiles = a.tiles_m * a.tiles_n;
-  const int xcd = blockIdx.x & 7, idx = blockIdx.x >> 3;               // the tiles of a strip share an L2
-  const int strip = idx / tiles * 8 + xcd, tile = idx % tiles;
+  // an eighth of the (strip, tile) pairs to each XCD, strip by strip: the tiles of a strip, which read the same rows, share an L2
+  const int64_t per = gridDim.x >> 3, item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  const int strip = (int)(item / tiles), tile = (int)(item % tiles);
   if (strip >= a.strips) return;
   const int m0 = tile / a.tiles_n * BM, n0 = tile % a.tiles_n * BN;
   const bool first_n = n0 == 0;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = (wave >> 1) * WM, wn = (wave & 1) * WN;
-  const int cw = tid & 31, rq = tid >> 5, steps = (int)(((a.n + BK - 1) / BK - strip + a.strips - 1) / a.strips);
+  // (half a wave writes both halves of 16 slots: 256 bytes on end, every bank once)
+  const int cw = (tid & 15) | ((tid >> 1) & 16), rq = ((tid >> 5) & 6) | ((tid >> 4) & 1), steps = (int)(((a.n + BK - 1) / BK - strip + a.strips - 1) / a.strips);
   // columns behind the last one: some other column's values, in rows or columns of the tile that nobody keeps
   const int ca = min(m0 + cw * WA, a.m - 1) / WA * WA, cb = min(n0 + cw * WB, a.k - 1) / WB * WB;
   // the last columns of an odd width are read from further left, and moved into place when they are laid down
@@ -365,19 +367,20 @@ __global__ __launch_bounds__(256) void checkpoint8_backward_kernel(back_args a) 
     }
   };
 
-  // Step i is multiplied out of buffer i mod 2 while step i + 1 is laid down in the other and step i + 2 is asked for.
-  back_regs<T, WA, WB> g;
-  fetch(g, 0);
-  lay_down(g, 0, lds[0]);
-  fetch(g, 1);
+  // Step i is multiplied out of buffer i mod 2 while step i + 1 is laid down in the other and step i + 3 is asked for.
+  back_regs<T, WA, WB> g0, g1;
+  fetch(g0, 0);
+  fetch(g1, 1);
+  lay_down(g0, 0, lds[0]);
+  fetch(g0, 2);
   __syncthreads();
   for (int i = 0; i < steps; i += 2) {
-    lay_down(g, i + 1, lds[1]);
-    fetch(g, i + 2);
+    lay_down(g1, i + 1, lds[1]);
+    fetch(g1, i + 3);
     multiply(lds[0]);
     __syncthreads();
-    lay_down(g, i + 2, lds[0]);
-    fetch(g, i + 3);
+    lay_down(g0, i + 2, lds[0]);
+    fetch(g0, i + 4);
     multiply(lds[1]);
     __syncthreads();
   }
@@ -469,9 +472,8 @@ row_grid rows_of(int64_t n, int k, int columns) {
   return g;
 }
 
-// Tiles of 128 columns, or 64 where that leaves fewer of them empty; strips so that some 512 workgroups run, of some 128
-// rows at least each, or 1024 where a strip still has 512 rows: more loads on their way at once against twice the partial
-// sums (1e6 rows, 128 -> 64, fp32, tanh: 149 against 163 us; 31882 rows, 136 -> 32: 20.7 against 19.9 us).
+// Tiles of 128 columns, or 64 where that leaves fewer of them empty; strips so that some 512 workgroups run, two a CU, of
+// some 128 rows at least each (1024: 1e6 rows, 128 -> 64, fp32, tanh 153 against 141 us, for the partial sums they add).
 int side_of(int columns) { return (columns + 127) / 128 * 2 > (columns + 63) / 64 ? 64 : 128; }
 struct back_plan {
   int bm, bn, tiles_m, tiles_n, strips;
@@ -484,10 +486,8 @@ back_plan plan_of(int64_t n, int k, int m) {
   p.tiles_m = (m + p.bm - 1) / p.bm;
   p.tiles_n = (k + p.bn - 1) / p.bn;
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
-  auto least = [](int64_t a, int64_t b) { return a < b ? a : b; };
-  int64_t strips = least((512 + tiles - 1) / tiles, (n + 127) / 128);
-  const int64_t more = least((1024 + tiles - 1) / tiles, n / 512);
-  if (strips < more) strips = more;
+  int64_t strips = (512 + tiles - 1) / tiles;
+  strips = strips < (n + 127) / 128 ? strips : (n + 127) / 128;
   p.strips = (int)strips;
   p.part = 0;
   p.part_b = (size_t)p.strips * tiles * p.bm * p.bn * 4;
@@ -497,7 +497,7 @@ back_plan plan_of(int64_t n, int k, int m) {
 
 template <typename T, int FMT, bool TANH, int PIECES, int BM, int BN, bool NARROW>
 int back_as(const back_plan &p, const back_args &a, T *d_w, T *d_b, hipStream_t stream) {
-  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, blocks = (int64_t)(p.strips + 7) / 8 * 8 * tiles;
+  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, blocks = (p.strips * tiles + 7) / 8 * 8;
   int log_strands = 0;
   while (log_strands < 6 && (2 << log_strands) <= p.strips) ++log_strands;
   const int per = 1024 >> log_strands;
