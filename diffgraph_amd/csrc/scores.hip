@@ -50,12 +50,27 @@ __global__ __launch_bounds__(256) void adjust_scores_kernel(score_args a) {
     }
   }
   const bool any = begin < end;
+  // the tile's scores are asked for first: they arrive while the history is counted
+  const T *src = (const T *)a.scores + row * a.stride + c0;
+  T *dst = (T *)a.out + row * a.out_stride + c0;
+  constexpr int N = kTile / (256 * VEC);
+  dg_vec<T, VEC> held[N];
+#pragma unroll
+  for (int v = 0; v < N; ++v) {
+    const int c = (v * 256 + threadIdx.x) * VEC;
+    if (c + VEC <= width) held[v] = dg_load_raw<VEC, 2>(src + c);
+  }
   if (any) {
-    for (int i = threadIdx.x; i < kTile; i += 256) had[i] = 0;
+    for (int i = 4 * threadIdx.x; i < kTile; i += 1024) *reinterpret_cast<uint4 *>(&had[i]) = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    for (int64_t i = begin + threadIdx.x; i < end; i += 256) {
-      const uint32_t c = (uint32_t)(a.col[i] - c0);
-      if (c < (uint32_t)width) atomicAdd(&had[c], 1u);      // (entries outside [0, items) are in no tile)
+    constexpr int U = 8;                                    // entries on their way at a time
+    for (int64_t i = begin + threadIdx.x; i < end; i += 256 * U) {
+      uint32_t c[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) c[u] = (uint32_t)(a.col[min(i + 256 * u, end - 1)] - c0);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i + 256 * u < end && c[u] < (uint32_t)width) atomicAdd(&had[c[u]], 1u);   // (entries outside [0, items) are in no tile)
     }
     __syncthreads();
   }
@@ -68,13 +83,15 @@ __global__ __launch_bounds__(256) void adjust_scores_kernel(score_args a) {
     if ((uint64_t)m < (uint64_t)a.n_masks) mask = a.allowed + m * a.allowed_stride;
   }
   const float *bias = a.bias ? a.bias + row * a.bias_stride : nullptr;
-  const T *src = (const T *)a.scores + row * a.stride + c0;
-  T *dst = (T *)a.out + row * a.out_stride + c0;
-  for (int c = threadIdx.x * VEC; c < width; c += 256 * VEC) {
+#pragma unroll
+  for (int v = 0; v < N; ++v) {
+    const int c = (v * 256 + threadIdx.x) * VEC;
+    if (c >= width) break;
     const bool whole = c + VEC <= width;
     float s[VEC], more[VEC] = {};
     if (whole) {
-      dg_load_unaligned<VEC>(src + c, s);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) s[e] = dg_widen(held[v].v[e]);
       if (bias) dg_load_unaligned<VEC>(bias + c0 + c, more);
     } else {
 #pragma unroll
