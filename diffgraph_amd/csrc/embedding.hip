@@ -27,14 +27,14 @@ __global__ __launch_bounds__(256) void embedding_lookup_kernel(const T *__restri
   for (int c = (threadIdx.x % GL) * VEC; c < dim; c += GL * VEC) {
     float f[VEC];
     if (ok) {
-      dg_load<VEC>(src + c, f);
+      dg_load_unaligned<VEC>(src + c, f);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) f[e] *= scale;
     } else {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) f[e] = __builtin_nanf("");
     }
-    dg_store<VEC>(dst + c, f);
+    dg_store_unaligned<VEC>(dst + c, f);
   }
 }
 
@@ -349,7 +349,7 @@ __device__ __forceinline__ void zero_unnamed_rows(int64_t block, const uint32_t 
   for (int r = g; r < rows; r += 256 / GL) {
     if (named[r]) continue;
     T *dst = d_table + (r0 + r) * dim;
-    for (int c = l; c < steps; c += GL) dg_store<VEC>(dst + c * VEC, zero);
+    for (int c = l; c < steps; c += GL) dg_store_unaligned<VEC>(dst + c * VEC, zero);
   }
 }
 
@@ -377,13 +377,13 @@ __global__ __launch_bounds__(256) void embedding_runs_kernel(const T *__restrict
   auto flush = [&](bool goes_on) {
     if (!live || cur >= n_rows) return;
     if (open || goes_on) {
-      dg_store<VEC>(slab + (size_t)(2 * c + (open ? 0 : 1)) * dim + col, acc);
-      if (!open && col == 0) crossing[atomicAdd(n_crossing, 1u)] = (uint32_t)c;
+      dg_store_unaligned<VEC>(slab + (size_t)(2 * c + (open ? 0 : 1)) * dim + col, acc);
+      if (!open && col == 0 && crossing) crossing[atomicAdd(n_crossing, 1u)] = (uint32_t)c;
     } else {
       float f[VEC];
 #pragma unroll
       for (int v = 0; v < VEC; ++v) f[v] = acc[v] * scale;
-      dg_store<VEC>(d_table + (size_t)cur * dim + col, f);
+      dg_store_unaligned<VEC>(d_table + (size_t)cur * dim + col, f);
     }
   };
   constexpr int U = 8;
@@ -398,7 +398,7 @@ __global__ __launch_bounds__(256) void embedding_runs_kernel(const T *__restrict
     dg_vec<T, VEC> row[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (live && i + u < e) row[u] = dg_load_raw<VEC, 16>(d_out + (int64_t)p[u] * stride + col);
+      if (live && i + u < e) row[u] = dg_load_raw<VEC, 2>(d_out + (int64_t)p[u] * stride + col);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (i + u >= e) break;
@@ -418,7 +418,82 @@ __global__ __launch_bounds__(256) void embedding_runs_kernel(const T *__restrict
   flush(e < n && keys[e] == cur);
 }
 
-// The runs that cross from chunk to chunk, 64 columns of one at a time: 16 strands of every 16th part, the strands added in
+// Long lists: the parts that chunks left are first added up over kFold neighbouring chunks, as if those were one.  A run that
+// begins and ends among them is written to its row, one that crosses their border leaves its part in their two places of the
+// next slab (and is listed).  16 lanes take 64 columns; the parts of eight chunks are on their way at a time.
+// A million ids that are all the same, 64 columns: 140 us against 532 us without; 2048 chunks of 65536 ids that fall off like
+// one over their rank, 1024 columns: 18 against 13 us, so shorter lists go without.
+constexpr int kFold = 16, kFoldMin = 2048;
+template <typename T>
+__global__ __launch_bounds__(256) void embedding_fold_kernel(const uint32_t *__restrict__ keys, int64_t n, uint32_t n_rows, int dim, int chunk,
+                                                             int64_t n_chunks, float scale, const float *__restrict__ slab,
+                                                             T *__restrict__ d_table, float *__restrict__ next_slab,
+                                                             uint32_t *__restrict__ crossing, uint32_t *__restrict__ n_crossing) {
+  const int64_t f = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4), c0 = f * kFold, c1 = min(c0 + kFold, n_chunks);
+  if (c0 >= n_chunks) return;
+  const int col = blockIdx.y * 64 + (threadIdx.x & 15) * 4, live = max(0, min(4, dim - col));
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  bool from_before = true;                                  // the run at hand began before these chunks
+  auto load = [&](int64_t place, float (&v)[4]) {
+    const float *src = slab + (size_t)place * dim + col;
+    if (live == 4) {
+      dg_load_unaligned<4>(src, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = e < live ? src[e] : 0.f;
+    }
+  };
+  auto leave = [&](uint32_t key, bool goes_on) {
+    if (from_before || goes_on) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < live) next_slab[(size_t)(2 * f + (from_before ? 0 : 1)) * dim + col + e] = acc[e];
+      if (!from_before && col == 0) crossing[atomicAdd(n_crossing, 1u)] = (uint32_t)f;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < live) d_table[(size_t)key * dim + col + e] = dg_round<T>(acc[e] * scale);
+    }
+  };
+  constexpr int U = 8;
+  for (int64_t c = c0; c < c1; c += U) {
+    uint32_t before[U], first[U], last[U], after[U];
+    float head[U][4], tail[U][4];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t b = min(c + u, c1 - 1) * chunk, e = min(b + chunk, n);
+      before[u] = b ? keys[b - 1] : n_rows;
+      first[u] = keys[b];
+      last[u] = keys[e - 1];
+      after[u] = e < n ? keys[e] : n_rows;                  // (n_rows: the key of what takes no gradient, and leaves no part)
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t at = 2 * min(c + u, c1 - 1);
+      if (before[u] == first[u] && first[u] < n_rows) load(at, head[u]);
+      if (last[u] == after[u] && last[u] < n_rows) load(at + 1, tail[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (c + u >= c1) break;
+      const bool open = before[u] == first[u] && first[u] < n_rows, goes_on = last[u] == after[u] && last[u] < n_rows;
+      const bool through = open && goes_on && first[u] == last[u];      // nothing but the run at hand in this chunk
+      if (open) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += head[u][e];
+        if (!through) leave(first[u], false);
+      }
+      if (goes_on && !through) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = tail[u][e];
+        from_before = false;
+      }
+      if (c + u == c1 - 1 && goes_on) leave(last[u], true);
+    }
+  }
+}
+
+// The runs that cross from chunk to chunk (or from fold to fold), 64 columns of one at a time: 16 strands of every 16th part, the strands added in
 // order.  A workgroup takes every so many of them from the list.
 constexpr int kCrossCols = 64;
 template <typename T>
@@ -448,6 +523,7 @@ __global__ __launch_bounds__(256) void embedding_crossing_kernel(const uint32_t 
     __syncthreads();
     const int64_t last = last_chunk;
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
     for (int64_t k = c + g; k <= last; k += 16) {
       const float *src = slab + (size_t)(2 * k + (k == c ? 1 : 0)) * dim + col;
       if (col + 4 <= dim) {
@@ -474,28 +550,31 @@ __global__ __launch_bounds__(256) void embedding_crossing_kernel(const uint32_t 
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------------
+int type_size(int dtype) { return dtype == DG_F32 ? 4 : (dtype == DG_BF16 || dtype == DG_F16) ? 2 : 0; }
 constexpr int kMaxIpt = 16;
 int items_per_thread(int64_t n) { return n <= 256 * 256 * 4 ? 4 : kMaxIpt; }
 
-// Entries of a chunk: short ones while the list is short (every CU gets some), longer ones as it grows.
-int chunk_of(int64_t n, int dim) {
+// Entries of a chunk: as many as leave some 4096 waves (16 a CU), 8 to 256.  Short chunks are more loads on their way at
+// once, and more partial sums (65536 x 1024 bf16: 16 entries 118 us, 32: 103, 64: 114 for the runs and those that cross).
+int chunk_of(int64_t n, int dim, int elem) {
+  const int lanes = (dim * elem + 15) / 16;
   int c = 8;
-  while (c < 256 && n / c > 2048) c <<= 1;
+  while (c < 256 && (n / c * lanes > 4096 * 64 || (c < 16 && n / c > 2048))) c <<= 1;
   return c;
 }
 
 struct grad_plan {
-  int64_t n_blocks, n_chunks;
+  int64_t n_blocks, n_chunks, folds;   // (folds: 0 where the chunks' parts are added up at once)
   int ipt, chunk, passes, bits;     // bits of the id's range
   bool ranked;
-  size_t keys, pos, counts, totals, crossing, slab, bytes;   // offsets (two key and position lists)
+  size_t keys, pos, counts, totals, crossing, slab, folded, bytes;   // offsets (two key and position lists)
 };
 
-grad_plan plan_of(int64_t n_ids, int64_t n_rows, int dim) {
+grad_plan plan_of(int64_t n_ids, int64_t n_rows, int dim, int elem) {
   grad_plan p;
   p.ipt = items_per_thread(n_ids);
   p.n_blocks = (n_ids + 256 * p.ipt - 1) / (256 * p.ipt);
-  p.chunk = chunk_of(n_ids, dim);
+  p.chunk = chunk_of(n_ids, dim, elem);
   p.n_chunks = (n_ids + p.chunk - 1) / p.chunk;
   p.bits = 1;
   while (p.bits < 32 && (n_rows >> p.bits) != 0) ++p.bits;     // keys 0 .. n_rows
@@ -509,13 +588,11 @@ grad_plan plan_of(int64_t n_ids, int64_t n_rows, int dim) {
   p.counts = at; at += p.ranked ? 0 : (((size_t)p.n_blocks << kMaxDigit) * 4 + 255) & ~(size_t)255;
   p.totals = at; at += p.ranked ? 0 : (size_t)4 << kMaxDigit;
   p.crossing = at; at += ((size_t)p.n_chunks * 4 + 4 + 255) & ~(size_t)255;    // their number, then the chunks
-  p.slab = at; at += (size_t)p.n_chunks * 2 * dim * 4;
+  p.slab = at; at += ((size_t)p.n_chunks * 2 * dim * 4 + 255) & ~(size_t)255;
+  p.folds = p.n_chunks > kFoldMin ? (p.n_chunks + kFold - 1) / kFold : 0;
+  p.folded = at; at += (size_t)p.folds * 2 * dim * 4;
   p.bytes = at;
   return p;
-}
-
-bool aligned(const void *p, int64_t stride, int dim, int elem) {
-  return ((uintptr_t)p | (uintptr_t)(stride * elem) | (uintptr_t)((int64_t)dim * elem)) % 16 == 0;
 }
 
 int lanes_for(int steps) { return steps > 32 ? 64 : steps > 16 ? 32 : 16; }
@@ -533,43 +610,46 @@ int lookup_as(const void *table, int64_t n_rows, int64_t stride, int dim, const 
 
 template <typename T, int VEC, int GL>
 int grad_as(const grad_plan &p, const void *d_out, int64_t stride, const uint32_t *keys, const uint32_t *pos, int64_t n, int64_t n_rows,
-            int dim, float scale, void *d_table, float *slab, uint32_t *crossing, hipStream_t stream) {
+            int dim, float scale, void *d_table, float *slab, float *folded, uint32_t *crossing, hipStream_t stream) {
   const unsigned chunk_blocks = (unsigned)((p.n_chunks + 256 / GL - 1) / (256 / GL));
   const int cols = (dim + GL * VEC - 1) / (GL * VEC);
   const int64_t zero_blocks = (n_rows + kZeroRows - 1) / kZeroRows;
   const dim3 grid(chunk_blocks + (unsigned)((zero_blocks + cols - 1) / cols), cols);
   hipLaunchKernelGGL((embedding_runs_kernel<T, VEC, GL>), grid, dim3(256), 0, stream, (const T *)d_out, stride, dim, keys, pos, n,
-                     (uint32_t)n_rows, p.chunk, chunk_blocks, scale, (T *)d_table, slab, crossing + 1, crossing);
+                     (uint32_t)n_rows, p.chunk, chunk_blocks, scale, (T *)d_table, slab, p.folds ? nullptr : crossing + 1, crossing);
   DG_HIP(hipGetLastError());
   if (p.n_chunks < 2) return 0;      // nothing to cross into
-  const int64_t items = p.n_chunks * ((dim + kCrossCols - 1) / kCrossCols);
+  const unsigned col_blocks = (unsigned)((dim + kCrossCols - 1) / kCrossCols);
+  if (p.folds) {
+    hipLaunchKernelGGL((embedding_fold_kernel<T>), dim3((unsigned)((p.folds + 15) / 16), col_blocks), dim3(256), 0, stream, keys, n,
+                       (uint32_t)n_rows, dim, p.chunk, p.n_chunks, scale, slab, (T *)d_table, folded, crossing + 1, crossing);
+    DG_HIP(hipGetLastError());
+  }
+  const int64_t items = (p.folds ? p.folds : p.n_chunks) * col_blocks;
   hipLaunchKernelGGL((embedding_crossing_kernel<T>), dim3((unsigned)(items < 2048 ? items : 2048)), dim3(256), 0, stream, keys, n, dim,
-                     p.chunk, scale, slab, crossing + 1, crossing, (T *)d_table);
+                     p.folds ? p.chunk * kFold : p.chunk, scale, p.folds ? folded : slab, crossing + 1, crossing, (T *)d_table);
   DG_HIP(hipGetLastError());
   return 0;
 }
 
-// The widest load that rows of this width and alignment allow (16 bytes, or one element), and the lanes a row takes.
-#define DG_BY_LANES(FN, T, VEC, steps, ...)                 \
-  switch (lanes_for(steps)) {                               \
+// The widest loads, of up to 16 bytes, that cut a row into whole ones, and the lanes a row takes.
+#define DG_BY_LANES(FN, T, VEC, dim, ...)                   \
+  switch (lanes_for((dim) / (VEC))) {                       \
     case 64: return FN<T, VEC, 64>(__VA_ARGS__);            \
     case 32: return FN<T, VEC, 32>(__VA_ARGS__);            \
     default: return FN<T, VEC, 16>(__VA_ARGS__);            \
   }
-#define DG_BY_TYPE(FN, dtype, wide, dim, ...)                                              \
-  switch (dtype) {                                                                         \
-    case DG_F32:                                                                           \
-      if (wide) { DG_BY_LANES(FN, float, 4, ((dim) + 3) / 4, __VA_ARGS__) }                \
-      DG_BY_LANES(FN, float, 1, dim, __VA_ARGS__)                                          \
-    case DG_BF16:                                                                          \
-      if (wide) { DG_BY_LANES(FN, dg_bf16, 8, ((dim) + 7) / 8, __VA_ARGS__) }              \
-      DG_BY_LANES(FN, dg_bf16, 1, dim, __VA_ARGS__)                                        \
-    default:                                                                               \
-      if (wide) { DG_BY_LANES(FN, dg_f16, 8, ((dim) + 7) / 8, __VA_ARGS__) }               \
-      DG_BY_LANES(FN, dg_f16, 1, dim, __VA_ARGS__)                                         \
+#define DG_BY_WIDTH(FN, T, dim, ...)                                                          \
+  if ((dim) % (16 / (int)sizeof(T)) == 0) { DG_BY_LANES(FN, T, 16 / (int)sizeof(T), dim, __VA_ARGS__) } \
+  if ((dim) % (8 / (int)sizeof(T)) == 0) { DG_BY_LANES(FN, T, 8 / (int)sizeof(T), dim, __VA_ARGS__) }   \
+  if (sizeof(T) == 2 && (dim) % 2 == 0) { DG_BY_LANES(FN, T, 2, dim, __VA_ARGS__) }           \
+  DG_BY_LANES(FN, T, 1, dim, __VA_ARGS__)
+#define DG_BY_TYPE(FN, dtype, dim, ...)                     \
+  switch (dtype) {                                          \
+    case DG_F32: DG_BY_WIDTH(FN, float, dim, __VA_ARGS__)   \
+    case DG_BF16: DG_BY_WIDTH(FN, dg_bf16, dim, __VA_ARGS__) \
+    default: DG_BY_WIDTH(FN, dg_f16, dim, __VA_ARGS__)      \
   }
-
-int type_size(int dtype) { return dtype == DG_F32 ? 4 : (dtype == DG_BF16 || dtype == DG_F16) ? 2 : 0; }
 
 int check_sizes(const char *what, int64_t n_ids, int64_t n_rows, int dim, int dtype) {
   if (!type_size(dtype)) return dg_fail(DG_ERR_ARG, "%s: unknown element type %d", what, dtype);
@@ -587,14 +667,12 @@ extern "C" int dg_embedding_lookup(const void *table, int64_t n_rows, int64_t ro
   if (n_ids == 0) return 0;
   if (!table || !ids || !out) return dg_fail(DG_ERR_ARG, "dg_embedding_lookup: NULL argument");
   if (row_stride < 0) return dg_fail(DG_ERR_ARG, "dg_embedding_lookup: negative row stride");
-  const int z = type_size(dtype);
-  const bool wide = aligned(table, row_stride, dim, z) && aligned(out, dim, dim, z);
-  DG_BY_TYPE(lookup_as, dtype, wide, dim, table, n_rows, row_stride, dim, ids, ids_are_64, n_ids, scale, out, (hipStream_t)stream)
+  DG_BY_TYPE(lookup_as, dtype, dim, table, n_rows, row_stride, dim, ids, ids_are_64, n_ids, scale, out, (hipStream_t)stream)
 }
 
 extern "C" size_t dg_embedding_grad_workspace(int64_t n_ids, int64_t n_rows, int32_t dim) {
   if (n_ids < 0 || n_rows <= 0 || dim <= 0) return 0;
-  return plan_of(n_ids, n_rows, dim).bytes;
+  return plan_of(n_ids, n_rows, dim, 2).bytes;      // (of 16-bit rows: the shorter chunks, the larger workspace)
 }
 
 extern "C" int dg_embedding_grad(const void *d_out, int64_t row_stride, const void *ids, int32_t ids_are_64, int64_t n_ids, int64_t n_rows,
@@ -603,7 +681,7 @@ extern "C" int dg_embedding_grad(const void *d_out, int64_t row_stride, const vo
   if (const int rc = check_sizes("dg_embedding_grad", n_ids, n_rows, dim, dtype)) return rc;
   if (!d_table || (n_ids && (!d_out || !ids || !workspace))) return dg_fail(DG_ERR_ARG, "dg_embedding_grad: NULL argument");
   if (row_stride < 0) return dg_fail(DG_ERR_ARG, "dg_embedding_grad: negative row stride");
-  const grad_plan p = plan_of(n_ids, n_rows, dim);
+  const grad_plan p = plan_of(n_ids, n_rows, dim, type_size(dtype));
   if (n_ids && (workspace_bytes < p.bytes || ((uintptr_t)workspace & 15)))
     return dg_fail(DG_ERR_SIZE, "dg_embedding_grad: a 16-byte aligned workspace of %zu bytes is needed, got %zu", p.bytes, workspace_bytes);
   hipStream_t st = (hipStream_t)stream;
@@ -639,8 +717,6 @@ extern "C" int dg_embedding_grad(const void *d_out, int64_t row_stride, const vo
     }
     at ^= 1;
   }
-  const int z = type_size(dtype);
-  const bool wide = (!n_ids || aligned(d_out, row_stride, dim, z)) && aligned(d_table, dim, dim, z);
-  DG_BY_TYPE(grad_as, dtype, wide, dim, p, d_out, row_stride, keys[at], pos[at], n_ids, n_rows, dim, scale, d_table,
-             (float *)(ws + p.slab), crossing, st)
+  DG_BY_TYPE(grad_as, dtype, dim, p, d_out, row_stride, keys[at], pos[at], n_ids, n_rows, dim, scale, d_table,
+             (float *)(ws + p.slab), (float *)(ws + p.folded), crossing, st)
 }

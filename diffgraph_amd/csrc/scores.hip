@@ -67,7 +67,7 @@ __global__ __launch_bounds__(256) void adjust_scores_kernel(score_args a) {
     for (int64_t i = begin + threadIdx.x; i < end; i += 256 * U) {
       uint32_t c[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) c[u] = (uint32_t)(a.col[min(i + 256 * u, end - 1)] - c0);
+      for (int u = 0; u < U; ++u) c[u] = (uint32_t)a.col[min(i + 256 * u, end - 1)] - (uint32_t)c0;
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (i + 256 * u < end && c[u] < (uint32_t)width) atomicAdd(&had[c[u]], 1u);   // (entries outside [0, items) are in no tile)

@@ -765,8 +765,8 @@ int dg_adjust_scores(const dg_score_task *task, void *stream);
  *   dg_checkpoint8_backward  of y = x . w^T + b (y_kept NULL) or y = tanh(x . w^T + b), from d_y [n][m], what was kept of
  *                            x [n][k] and, with tanh, of y [n][m] (both in `format`):
  *                              d_z = d_y (1 - y y) (written with tanh only), d_w[m][k] = d_z^T . x, d_b[m] = column sums
- *                            in fp32 over strips of rows added in strip order, every output rounded once to dtype.  An
- *                            infinity in d_y gives NaN in its column of d_w
+ *                            in fp32 over strips of rows added in strip order, every output rounded once to dtype.  A
+ *                            column of d_y with an infinity or a NaN in it gives no finite row of d_w
  * dtype (x, out, d_y, d_z, d_w, d_b): DG_F32 / DG_BF16 / DG_F16; row_stride: elements between the rows of x / d_y (of d_y:
  * m to 2^24).  Kept bytes and workspace: DEVICE, 16-byte aligned.  workspace: dg_checkpoint8_backward_workspace bytes,
  * contents irrelevant; calls that may run at the same time need one each.
