@@ -148,7 +148,7 @@ __global__ __launch_bounds__(256) void head_bwd_entries_kernel(const float *ui, 
     const int e = l == 2 ? n_batch + b : b;                 // index in the row's list (ancs; poss then negs)
     atomicMax(tag + trow, (l == 0 ? n_batch : 2 * n_batch) - e);
     const int k = atomicAdd(cnt + trow, 1);
-    if (k < kSlots) slots[(size_t)trow * kSlots + k] = e;
+    if ((unsigned)k < (unsigned)kSlots) slots[(size_t)trow * kSlots + k] = e;   // (a count that was never cleared writes nowhere)
     idx32[l * n_batch + b] = l == 0 ? (int)a : (int)(l == 1 ? p : n);
   }
 }
@@ -172,7 +172,10 @@ __global__ __launch_bounds__(256) void head_scatter_kernel(int n_batch, int n_us
   const int trow = user ? row : n_user + row, c = cnt[trow];
   if (c != 1 && m - tag[trow] != e) return;  // not the only entry naming this row, nor the first of several
   if (c > kSlots) {
-    if (l == 0) heavy[1 + atomicAdd(heavy, 1)] = e_all;
+    if (l == 0) {
+      const int at = atomicAdd(heavy, 1);
+      if (at < n_batch) heavy[1 + at] = e_all;
+    }
     return;
   }
   const f32x4 *G = reinterpret_cast<const f32x4 *>(scratch) + (user ? (size_t)0 : (size_t)n_batch * 16);
@@ -193,7 +196,7 @@ __global__ __launch_bounds__(256) void head_scatter_kernel(int n_batch, int n_us
 #pragma unroll
     for (int k = 1; k < kSlots; ++k)   // s[0] == e, the first entry
       if (k < c) {
-        acc += G[(size_t)s[k] * 16 + l];
+        acc += G[(size_t)min((unsigned)s[k], (unsigned)(m - 1)) * 16 + l];
         n_loss += (user || s[k] < n_batch) ? 1 : 0;
       }
   }
@@ -260,6 +263,26 @@ __global__ __launch_bounds__(16 * kHeavyRuns) void head_heavy_kernel(int n_batch
   }
 }
 
+// Zeros, 16 bytes a thread and step; the bytes in front of the first and behind the last whole 16 one by one.  A kernel of
+// its own and not the runtime's memset: recorded into a HIP graph that is a memset node, and those have been seen to leave
+// memory as it was on replays after the first -- here the counters that slots are indexed by.
+__global__ __launch_bounds__(256) void clear_kernel(uint8_t *dst, size_t head, size_t quads, size_t tail) {
+  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+  uint4 *mid = reinterpret_cast<uint4 *>(dst + head);
+  for (size_t q = i; q < quads; q += (size_t)gridDim.x * 256) mid[q] = make_uint4(0, 0, 0, 0);
+  if (i < head) dst[i] = 0;
+  if (i < tail) dst[head + 16 * quads + i] = 0;
+}
+
+int clear_bytes(void *dst, size_t bytes, hipStream_t stream) {
+  const size_t to_16 = (16 - ((uintptr_t)dst & 15)) & 15, head = to_16 < bytes ? to_16 : bytes;
+  const size_t quads = (bytes - head) / 16, tail = bytes - head - 16 * quads, blocks = (quads + 1023) / 1024;
+  hipLaunchKernelGGL(clear_kernel, dim3((unsigned)(blocks < 1 ? 1 : blocks < 1024 ? blocks : 1024)), dim3(256), 0, stream, (uint8_t *)dst, head,
+                     quads, tail);
+  DG_HIP(hipGetLastError());
+  return 0;
+}
+
 // flags[row] = 1 for every table row a batch entry names (users: ancs; items, behind the users: poss and negs)
 __global__ __launch_bounds__(256) void mark_rows_kernel(const int64_t *__restrict__ ancs, const int64_t *__restrict__ poss,
                                                         const int64_t *__restrict__ negs, int n_batch, int n_user, int n_item,
@@ -315,7 +338,7 @@ extern "C" int dg_active_rows(const int64_t *ancs, const int64_t *poss, const in
   if (!ancs || !poss || !negs || !flags || !rows_u || !rows_i || !counts) return dg_fail(DG_ERR_ARG, "dg_active_rows: NULL argument");
   if (n_batch <= 0 || n_batch > kMaxBatch) return dg_fail(DG_ERR_SIZE, "dg_active_rows: n_batch must be in [1,%d] (got %d)", kMaxBatch, n_batch);
   if (n_user <= 0 || n_item <= 0) return dg_fail(DG_ERR_ARG, "dg_active_rows: bad sizes");
-  DG_HIP(hipMemsetAsync(flags, 0, ((size_t)n_user + (size_t)n_item) * sizeof(int32_t), (hipStream_t)stream));
+  if (const int rc = clear_bytes(flags, ((size_t)n_user + (size_t)n_item) * sizeof(int32_t), (hipStream_t)stream)) return rc;
   hipLaunchKernelGGL(mark_rows_kernel, dim3((3 * n_batch + 255) / 256), dim3(256), 0, (hipStream_t)stream, ancs, poss, negs, n_batch,
                      n_user, n_item, flags);
   const int blocks_u = (n_user + kCompact - 1) / kCompact, blocks_i = (n_item + kCompact - 1) / kCompact;
@@ -383,11 +406,9 @@ extern "C" int dg_rec_head_bwd(const float *ui, const float *out_u, const float 
 }
 
 // The zeroed buffer dg_rec_head_bwd starts from (autograd's zero-initialised gradient tables of the three batch gathers,
-// DiffGraph-Rec/Model.py:101-104), cleared by the runtime's memset on the caller's stream -- recorded into a HIP graph
-// it is a memset node, not a kernel.
+// DiffGraph-Rec/Model.py:101-104), cleared on the caller's stream.
 extern "C" int dg_clear(void *dst, size_t bytes, void *stream) {
   if (!dst && bytes) return dg_fail(DG_ERR_ARG, "dg_clear: NULL buffer");
   if (bytes == 0) return 0;
-  DG_HIP(hipMemsetAsync(dst, 0, bytes, (hipStream_t)stream));
-  return 0;
+  return clear_bytes(dst, bytes, (hipStream_t)stream);
 }

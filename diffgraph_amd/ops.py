@@ -570,7 +570,7 @@ def active_rows_buffers(n_batch: int, n: int, device):
 
 
 def clear_table(t: torch.Tensor) -> None:
-    """Zeroes a table with the runtime's memset on the current stream (a memset node in a recorded step)."""
+    """Zeroes a table on the current stream."""
     rc = _lib.load().dg_clear(t.data_ptr(), t.numel() * t.element_size(), _lib.stream_ptr(t.device))
     _lib.check(rc, "dg_clear")
 

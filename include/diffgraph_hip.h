@@ -541,7 +541,7 @@ int dg_rec_head_fwd(const float *ui, const float *out_u, const float *out_i, con
 int dg_rec_head_reduce(const float *entries_f, const double *entries_d, int32_t n_batch, double batch_div,
                        double reg_coef, double *results, void *stream);
 
-/* Clears `bytes` bytes at dst on `stream` (hipMemsetAsync): the zero state dg_rec_head_bwd's buffer has to be handed
+/* Clears `bytes` bytes at dst on `stream` (a kernel, also where it is recorded): the zero state dg_rec_head_bwd's buffer has to be handed
  * over in -- the zero-initialised gradient tables autograd creates for the batch gathers of DiffGraph-Rec/Model.py:101-104. */
 int dg_clear(void *dst, size_t bytes, void *stream);
 
