@@ -460,15 +460,17 @@ int check_sizes(const char *what, int64_t n, int64_t k, int fmt) {
 int64_t quads_of(int64_t n) { return (n + 3) / 4; }
 size_t scales_at(int64_t n, int k) { return (size_t)quads_of(n) * 4 * pitch_of(k); }
 
+constexpr int64_t kMostBlocks = 0xffffff;       // of 256 threads: a launch has fewer than 2^32 (2^35 elements fit for any k)
+
 struct row_grid {
   int lanes, quads_per_block;
-  unsigned blocks;
+  int64_t blocks;
 };
 row_grid rows_of(int64_t n, int k, int columns) {
   row_grid g;
   g.lanes = kGroup / columns * groups_of(k);
   g.quads_per_block = g.lanes >= 256 ? 1 : 256 / g.lanes;
-  g.blocks = (unsigned)((quads_of(n) + g.quads_per_block - 1) / g.quads_per_block);
+  g.blocks = (quads_of(n) + g.quads_per_block - 1) / g.quads_per_block;
   return g;
 }
 
@@ -502,7 +504,7 @@ int back_as(const back_plan &p, const back_args &a, T *d_w, T *d_b, hipStream_t 
   while (log_strands < 6 && (2 << log_strands) <= p.strips) ++log_strands;
   const int per = 1024 >> log_strands;
   const int64_t sums = tiles * (BM * BN / per) + ((int64_t)p.tiles_m * BM + per - 1) / per;
-  if (blocks > 0x7fffffff || sums > 0x7fffffff) return dg_fail(DG_ERR_SIZE, "dg_checkpoint8_backward: a weight of %d x %d is too large", a.m, a.k);
+  if (blocks > kMostBlocks || sums > kMostBlocks) return dg_fail(DG_ERR_SIZE, "dg_checkpoint8_backward: a weight of %d x %d is too large", a.m, a.k);
   if (p.strips) {
     hipLaunchKernelGGL((checkpoint8_backward_kernel<T, FMT, TANH, PIECES, BM, BN, NARROW>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
     DG_HIP(hipGetLastError());
@@ -559,9 +561,10 @@ extern "C" int dg_checkpoint8(const void *x, int64_t row_stride, int64_t n, int3
   if (!x || !kept) return dg_fail(DG_ERR_ARG, "dg_checkpoint8: NULL argument");
   if ((uintptr_t)kept & 15) return dg_fail(DG_ERR_ARG, "dg_checkpoint8: the kept bytes must be 16-byte aligned");
   const row_grid g = rows_of(n, k, 16 / type_size(dtype));
+  if (g.blocks > kMostBlocks) return dg_fail(DG_ERR_SIZE, "dg_checkpoint8: %lld rows of %d columns are too many", (long long)n, k);
   uint8_t *codes = (uint8_t *)kept, *scales = codes + scales_at(n, k);
 #define DG_KEEP(T, F)                                                                                                               \
-  hipLaunchKernelGGL((checkpoint8_kernel<T, F, 16 / sizeof(T)>), dim3(g.blocks), dim3(256), 0, (hipStream_t)stream, (const T *)x, row_stride, n, k, \
+  hipLaunchKernelGGL((checkpoint8_kernel<T, F, 16 / sizeof(T)>), dim3((unsigned)g.blocks), dim3(256), 0, (hipStream_t)stream, (const T *)x, row_stride, n, k, \
                      pitch_of(k), g.lanes, g.quads_per_block, codes, scales)
   DG_BY_TYPE_AND_FORMAT(DG_KEEP, dtype, format)
 #undef DG_KEEP
@@ -576,9 +579,10 @@ extern "C" int dg_checkpoint8_values(const void *kept, int64_t n, int32_t k, int
   if (!kept || !out) return dg_fail(DG_ERR_ARG, "dg_checkpoint8_values: NULL argument");
   if ((uintptr_t)kept & 15) return dg_fail(DG_ERR_ARG, "dg_checkpoint8_values: the kept bytes must be 16-byte aligned");
   const row_grid g = rows_of(n, k, 4);
+  if (g.blocks > kMostBlocks) return dg_fail(DG_ERR_SIZE, "dg_checkpoint8_values: %lld rows of %d columns are too many", (long long)n, k);
   const uint8_t *codes = (const uint8_t *)kept, *scales = codes + scales_at(n, k);
 #define DG_READ(T, F)                                                                                                           \
-  hipLaunchKernelGGL((checkpoint8_values_kernel<T, F>), dim3(g.blocks), dim3(256), 0, (hipStream_t)stream, codes, scales, n, k, \
+  hipLaunchKernelGGL((checkpoint8_values_kernel<T, F>), dim3((unsigned)g.blocks), dim3(256), 0, (hipStream_t)stream, codes, scales, n, k, \
                      pitch_of(k), g.lanes, g.quads_per_block, (T *)out)
   DG_BY_TYPE_AND_FORMAT(DG_READ, dtype, format)
 #undef DG_READ

@@ -600,11 +600,14 @@ int lanes_for(int steps) { return steps > 32 ? 64 : steps > 16 ? 32 : 16; }
 template <typename T, int VEC, int GL>
 int lookup_as(const void *table, int64_t n_rows, int64_t stride, int dim, const void *ids, int ids64, int64_t n, float scale, void *out,
               hipStream_t stream) {
-  const int64_t blocks = (n + 256 / GL - 1) / (256 / GL);
-  if (blocks > 0x7fffffff) return dg_fail(DG_ERR_SIZE, "dg_embedding_lookup: too many ids");
-  hipLaunchKernelGGL((embedding_lookup_kernel<T, VEC, GL>), dim3((unsigned)blocks), dim3(256), 0, stream, (const T *)table, n_rows, stride,
-                     dim, ids, ids64, n, scale, (T *)out);
-  DG_HIP(hipGetLastError());
+  constexpr int64_t kMost = (int64_t)(1 << 22) * (256 / GL);      // (2^30 threads a launch: 2^32 are its limit)
+  for (int64_t first = 0; first < n; first += kMost) {
+    const int64_t some = n - first < kMost ? n - first : kMost;
+    hipLaunchKernelGGL((embedding_lookup_kernel<T, VEC, GL>), dim3((unsigned)((some + 256 / GL - 1) / (256 / GL))), dim3(256), 0, stream,
+                       (const T *)table, n_rows, stride, dim, (const char *)ids + first * (ids64 ? 8 : 4), ids64, some, scale,
+                       (T *)out + first * dim);
+    DG_HIP(hipGetLastError());
+  }
   return 0;
 }
 
@@ -681,6 +684,7 @@ extern "C" int dg_embedding_grad(const void *d_out, int64_t row_stride, const vo
   if (const int rc = check_sizes("dg_embedding_grad", n_ids, n_rows, dim, dtype)) return rc;
   if (!d_table || (n_ids && (!d_out || !ids || !workspace))) return dg_fail(DG_ERR_ARG, "dg_embedding_grad: NULL argument");
   if (row_stride < 0) return dg_fail(DG_ERR_ARG, "dg_embedding_grad: negative row stride");
+  if (n_rows > (1 << 29)) return dg_fail(DG_ERR_SIZE, "dg_embedding_grad: at most 2^29 rows");      // (4 threads a row, 2^32 in all)
   const grad_plan p = plan_of(n_ids, n_rows, dim, type_size(dtype));
   if (n_ids && (workspace_bytes < p.bytes || ((uintptr_t)workspace & 15)))
     return dg_fail(DG_ERR_SIZE, "dg_embedding_grad: a 16-byte aligned workspace of %zu bytes is needed, got %zu", p.bytes, workspace_bytes);

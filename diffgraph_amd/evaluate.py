@@ -90,6 +90,7 @@ def all_rank_topk(usrEmbeds: torch.Tensor, itmEmbeds: torch.Tensor, users: torch
     return top_val, top_idx
 
 
+@torch.no_grad()
 def recommend(usrEmbeds: torch.Tensor, itmEmbeds: torch.Tensor, users: torch.Tensor, data: AllRankTestData, topk: int = 20, *,
               exclude: bool = True, repetition=None, frequency=None, presence=None, bias=None, allowed=None, allowed_rows=None,
               batch: int = 1024):
@@ -118,7 +119,6 @@ def recommend(usrEmbeds: torch.Tensor, itmEmbeds: torch.Tensor, users: torch.Ten
             raise DiffGraphHipError(f"{nm}: expected one value for each of {n} users")
     if bias is not None and bias.dim() != 1:
         raise DiffGraphHipError(f"bias: expected shape [{n_item}]")
-    usrEmbeds, itmEmbeds = usrEmbeds.detach(), itmEmbeds.detach()
     top_val = torch.empty((n, topk), dtype=usrEmbeds.dtype, device=usrEmbeds.device)
     top_idx = torch.empty((n, topk), dtype=torch.int32, device=usrEmbeds.device)
     for b in range(0, n, batch):

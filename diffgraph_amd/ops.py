@@ -991,6 +991,8 @@ def _rows(x: torch.Tensor, name: str) -> torch.Tensor:
         raise DiffGraphHipError(f"{name}: rows have no columns")
     if x.shape[1] > 1 and x.stride(1) != 1 or x.stride(0) < 0:
         raise DiffGraphHipError(f"{name}: the elements of a row must lie next to each other (strides {tuple(x.stride())})")
+    if max(x.shape) > 0x7fffffff:
+        raise DiffGraphHipError(f"{name}: at most 2^31 - 1 rows and columns, got {tuple(x.shape)}")
     return x
 
 
@@ -1007,7 +1009,7 @@ def embedding_lookup(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0)
     _rows(table, "table")
     ids = _ids(ids, table.device)
     n, dim = table.shape
-    if n < 1 and ids.numel():
+    if n < 1:
         raise DiffGraphHipError("table: has no rows to look up")
     dev = table.device
     out = torch.empty((*ids.shape, dim), dtype=table.dtype, device=dev)
@@ -1024,8 +1026,8 @@ def embedding_grad(d_out: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: f
     d_out [*ids.shape, width] whose id it is, in fp32 in the order of their positions (fixed chunks of the list sorted by
     token: the same bits on every run); zeros where there are none.  Ids equal to padding_idx or outside [0, n_rows) take
     no part."""
-    if not isinstance(d_out, torch.Tensor) or d_out.dim() < 1 or tuple(d_out.shape[:-1]) != tuple(ids.shape):
-        raise DiffGraphHipError(f"d_out: expected shape [*{tuple(ids.shape)}, width]")
+    if not isinstance(d_out, torch.Tensor) or not isinstance(ids, torch.Tensor) or d_out.dim() < 1 or d_out.shape[:-1] != ids.shape:
+        raise DiffGraphHipError("d_out: expected a tensor of shape [*ids.shape, width], ids a tensor")
     if n_rows < 1:
         raise DiffGraphHipError("n_rows: a table has at least one row")
     dim, dev = d_out.shape[-1], d_out.device
@@ -1081,8 +1083,11 @@ def adjust_scores(scores: torch.Tensor, *, history=None, rows: Optional[torch.Te
     presence: a number or float32 [rows].  bias: float32 [items] or [rows, items].  allowed: int32 words of 32 items, bit
     v % 32 of word v // 32 set where item v stays, [words] for all rows or [masks, words] with allowed_rows (int32 [rows]; a
     row whose number is not that of a mask has none; default: mask r for row r).  A row whose mask leaves nothing is all
-    `fill`.  out: where to (scores itself: in place)."""
+    `fill`.  out: where to (scores itself: in place).  Not recorded by autograd, so neither scores nor bias may ask for a gradient
+    where one is recorded."""
     _rows(scores, "scores")
+    if torch.is_grad_enabled() and (scores.requires_grad or bias is not None and bias.requires_grad):
+        raise DiffGraphHipError("scores, bias: adjust_scores is not recorded by autograd: detach them")
     n, items = scores.shape
     dev = scores.device
     if out is None:

@@ -700,7 +700,7 @@ int dg_spgemm_pattern_fill(const uint32_t *bitmap, int32_t n_rows, int32_t n_col
  *                         and ids equal to padding_idx (-1: none) take no part.
  * dtype: DG_F32 / DG_BF16 / DG_F16, for table, out, d_out and d_table alike.  row_stride: elements between the rows of
  * table / d_out (out and d_table are contiguous).  ids: DEVICE int64 (ids_are_64 != 0) or int32.  At most 2^31 - 1 ids,
- * 2^31 - 2 rows.  workspace: DEVICE, 16-byte aligned, dg_embedding_grad_workspace bytes, contents irrelevant; calls
+ * 2^31 - 2 rows (of a gradient: 2^29).  workspace: DEVICE, 16-byte aligned, dg_embedding_grad_workspace bytes, contents irrelevant; calls
  * that may run at the same time need one each.
  * ---------------------------------------------------------------------------------- */
 #define DG_F32 0
@@ -768,8 +768,9 @@ int dg_adjust_scores(const dg_score_task *task, void *stream);
  *                            in fp32 over strips of rows added in strip order, every output rounded once to dtype.  A
  *                            column of d_y with an infinity or a NaN in it gives no finite row of d_w
  * dtype (x, out, d_y, d_z, d_w, d_b): DG_F32 / DG_BF16 / DG_F16; row_stride: elements between the rows of x / d_y (of d_y:
- * m to 2^24).  Kept bytes and workspace: DEVICE, 16-byte aligned.  workspace: dg_checkpoint8_backward_workspace bytes,
- * contents irrelevant; calls that may run at the same time need one each.
+ * m to 2^24).  At most 2^31 - 1 rows of 2^20 columns, 2^35 elements in all.  Kept bytes and workspace: DEVICE, 16-byte
+ * aligned.  workspace: dg_checkpoint8_backward_workspace bytes, contents irrelevant; calls that may run at the same time
+ * need one each.
  * ---------------------------------------------------------------------------------- */
 #define DG_INT8 0
 #define DG_E4M3 1

@@ -233,6 +233,8 @@ def test_recommend(width, dtype):
     assert ev.recommend(usr, itm, users[:0], data, 3)[0].shape == (0, 3)
     odd = ev.recommend(usr, itm, torch.tensor([nu, 2], device=DEV), data, 3)
     assert bool(odd[0][0].isnan().all()) and bool(odd[0][1].isfinite().all())
+    leaves = ev.recommend(usr.clone().requires_grad_(), itm, users[:1], data, 1, bias=torch.zeros(ni, device=DEV, requires_grad=True))
+    assert torch.equal(leaves[1], one[1]) and not leaves[0].requires_grad
 
 
 @gpu

@@ -252,6 +252,26 @@ def test_on_another_stream_and_in_a_graph():
         assert all(torch.equal(a, b) for a, b in zip(out, call()))
 
 
+@gpu
+def test_two_calls_at_once_on_two_streams():
+    g = torch.Generator().manual_seed(14)
+    work = []
+    for n, m, k, dtype in ((20000, 64, 100, torch.float32), (3001, 130, 257, torch.bfloat16)):
+        x, y, d = (torch.randn(n, c, generator=g).to(DEV).to(dtype) for c in (k, m, m))
+        work.append((d, x, torch.tanh(y)))
+    run = lambda d, x, y: ops.checkpoint8_backward(d, ops.checkpoint8(x), ops.checkpoint8(y))  # noqa: E731
+    alone = [run(*w) for w in work]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(4):
+        for s, w, out in zip(streams, work, got):
+            with torch.cuda.stream(s):
+                out.append(run(*w))
+    torch.cuda.synchronize()
+    for want, outs in zip(alone, got):
+        assert all(torch.equal(a, b) for o in outs for a, b in zip(o, want))
+
+
 # ---- refusals (no GPU needed) ---------------------------------------------------------------------------------------
 def test_c_entry_refuses_bad_arguments():
     lib, p = _lib.load(), 1 << 20

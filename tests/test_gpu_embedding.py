@@ -204,6 +204,37 @@ def test_an_output_row_past_32_bits():
     assert bool((grad[-1] == 2).all()) and bool((grad[0] == 1).all()) and not bool(grad[1:-1].any())
 
 
+@gpu
+def test_more_ids_than_one_launch_takes():
+    """16 lanes an id at one column: more than 2^26 ids take a second launch."""
+    table = torch.tensor([[1.0], [2.0], [3.0]], dtype=torch.bfloat16, device=DEV)
+    ids = torch.zeros((1 << 26) + 37, dtype=torch.int32, device=DEV)
+    ids[::1 << 18] = 2
+    ids[-17:] = 1
+    rows = ops.embedding_lookup(table, ids)
+    assert bool((rows[-17:] == 2).all()) and bool((rows[::1 << 18] == 3).all())
+    assert rows.view(torch.int16).ne(table.view(torch.int16)[0, 0]).sum().item() == 257 + 17      # (the others: 1)
+
+
+@gpu
+def test_two_calls_at_once_on_two_streams():
+    g = torch.Generator().manual_seed(12)
+    work = []
+    for n, rows in ((50000, 3000), (7000, 90000)):
+        ids = torch.randint(0, rows, (n,), generator=g).to(DEV)
+        work.append((torch.randn(n, 96, generator=g).to(DEV), ids, rows))
+    alone = [ops.embedding_grad(*w) for w in work]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(4):
+        for s, w, out in zip(streams, work, got):
+            with torch.cuda.stream(s):
+                out.append(ops.embedding_grad(*w))
+    torch.cuda.synchronize()
+    for want, outs in zip(alone, got):
+        assert all(torch.equal(o, want) for o in outs)
+
+
 # ---- refusals (no GPU needed) ---------------------------------------------------------------------------------------
 def test_cpu_tensors_and_bad_types_are_refused():
     t, ids = torch.zeros(4, 8), torch.zeros(3, dtype=torch.int64)
@@ -213,6 +244,8 @@ def test_cpu_tensors_and_bad_types_are_refused():
         ops.embedding_grad(torch.zeros(3, 8), ids, 4)
     with pytest.raises(DiffGraphHipError, match="shape"):
         ops.embedding_grad(torch.zeros(2, 8), ids, 4)
+    with pytest.raises(DiffGraphHipError, match="ids a tensor"):
+        ops.embedding_grad(torch.zeros(3, 8), [0, 1, 2], 4)
     with pytest.raises(DiffGraphHipError, match="n_rows"):
         ops.embedding_grad(torch.zeros(3, 8), ids, 0)
     with pytest.raises(DiffGraphHipError, match="padding_idx"):
@@ -229,6 +262,8 @@ def test_c_entry_refuses_bad_arguments():
     assert lib.dg_embedding_lookup(some, 0, 8, 8, 0, some, 1, 2, 1.0, some, None) == -1
     assert lib.dg_embedding_lookup(some, 1 << 31, 8, 8, 0, some, 1, 2, 1.0, some, None) == -3
     assert lib.dg_embedding_lookup(some, 4, 8, 8, 0, some, 1, 0, 1.0, some, None) == 0           # nothing to look up
+    assert lib.dg_embedding_grad(some, 1, some, 1, 0, (1 << 29) + 1, 1, 0, 1.0, -1, some, some, 0, None) == -3
+    assert b"2^29" in lib.dg_last_error()
     need = lib.dg_embedding_grad_workspace(100, 4, 8)
     assert need > 0 and lib.dg_embedding_grad_workspace(-1, 4, 8) == 0
     assert lib.dg_embedding_grad(some, 8, some, 1, 100, 4, 8, 0, 1.0, -1, some, some, need - 1, None) == -3
@@ -240,6 +275,8 @@ def test_c_entry_refuses_bad_arguments():
 @gpu
 def test_wrong_layouts_are_refused():
     t, ids = torch.zeros(8, 4, device=DEV), torch.zeros(3, dtype=torch.int64, device=DEV)
+    with pytest.raises(DiffGraphHipError, match="no rows"):
+        ops.embedding_lookup(t[:0], ids[:0])
     for bad, what in ((t.t(), "next to each other"), (t.double(), "float32"), (t[0], "2-D")):
         with pytest.raises(DiffGraphHipError, match=what):
             ops.embedding_lookup(bad, ids)

@@ -242,3 +242,17 @@ def test_wrong_arguments_are_refused():
         ops.adjust_scores(s, out=torch.zeros(64, device=DEV).expand(2, 64))
     with pytest.raises(DiffGraphHipError, match="next to each other"):
         ops.adjust_scores(s.t())
+    with pytest.raises(DiffGraphHipError, match="2\\^31"):
+        ops.adjust_scores(torch.zeros(1, 1, dtype=torch.bfloat16, device=DEV).expand(1 << 31, 1))
+
+
+@gpu
+def test_tensors_that_ask_for_a_gradient():
+    """The call is not recorded: where a gradient would be lost, it is refused."""
+    s, b = torch.randn(2, 64, device=DEV, requires_grad=True), torch.zeros(64, device=DEV, requires_grad=True)
+    for scores, bias in ((s, None), (s * 2, None), (s.detach(), b)):
+        with pytest.raises(DiffGraphHipError, match="autograd"):
+            ops.adjust_scores(scores, bias=bias)
+        with torch.no_grad():
+            assert torch.equal(ops.adjust_scores(scores, bias=bias), scores)
+    assert torch.equal(ops.adjust_scores(s.detach(), bias=b.detach()), s.detach())
