@@ -8,6 +8,8 @@ Python classes that keep the reference's call signatures:
     Denoise, GaussianDiffusion        DiffGraph-Rec/Model.py:176-399
     rec.HGDM, nc.HGDM                 DiffGraph-Rec/Model.py:16-118, DiffGraph_NC/Model.py:18-108
     evaluate.AllRankTestData, testEpoch, calcRes   DiffGraph-Rec/DataHandler.py:250-272, main.py:136-187
+    evaluate.recommend                top items for some users, with penalties, biases and masks
+    layers.embedding, Embedding       DiffGraph-Rec/Model.py:101-104 for tables of any width
     sampling.PairwiseTrnData          DiffGraph-Rec/DataHandler.py:274-296
     train.Coach                       DiffGraph-Rec/main.py:34-215 (trainEpoch, testEpoch, run)
     train_nc.NCCoach                  DiffGraph_NC/main.py:333-449 (prepareModel, trainEpoch, testEpoch, run)
