@@ -204,6 +204,7 @@ SIGNATURES = {
 }
 
 _lib: Optional[C.CDLL] = None
+_torch = None          # (imported by the first launch)
 
 
 def load() -> C.CDLL:
@@ -250,17 +251,19 @@ def device_guard(device=None):
     return torch.cuda.device(device)
 
 
-def launch(device, fn, what: str, *args) -> None:
-    """fn(*args, stream) on `device` (a tensor's) and its current stream; raises on an error code.  Makes the device current
-    where it is not.  (torch's own lookups of the current device and stream, without the objects round them: the small
-    operators are bound by their host time.)"""
-    import torch
-    at = device.index
-    if at == torch._C._cuda_getDevice():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(at))
+def launch(at: int, fn, what: str, *args) -> None:
+    """fn(*args, stream) on GPU `at` and its current stream; raises on an error code.  Makes the GPU current where it is not.
+    (torch's own lookups of the current device and stream, without the objects round them: the small operators are bound by
+    their host time.)"""
+    global _torch
+    if _torch is None:
+        import torch
+        _torch = torch
+    if at == _torch._C._cuda_getDevice():
+        rc = fn(*args, _torch._C._cuda_getCurrentRawStream(at))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(at))
+        with _torch.cuda.device(at):
+            rc = fn(*args, _torch._C._cuda_getCurrentRawStream(at))
     if rc != 0:
         check(rc, what)
 

@@ -983,40 +983,43 @@ def nc_head_bwd(target, diff, w, ancs, label_out, entries, g_nll: torch.Tensor, 
 _ELEMENT = {torch.float32: _lib.DG_F32, torch.bfloat16: _lib.DG_BF16, torch.float16: _lib.DG_F16}
 
 
-def _rows(x: torch.Tensor, name: str) -> torch.Tensor:
-    """A [rows, width] GPU tensor of one of the element types, the elements of a row next to each other."""
+def _rows(x: torch.Tensor, name: str):
+    """(rows, width, pitch, element type) of a [rows, width] GPU tensor of one of the element types, the elements of a row
+    next to each other.  (Small calls are bound by their host time: each of torch's properties is asked for once.)"""
     if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype not in _ELEMENT or x.dim() != 2:
         raise DiffGraphHipError(f"{name}: expected a 2-D float32, bfloat16 or float16 tensor on the GPU")
-    if x.shape[1] < 1:
+    (n, width), (pitch, step) = x.shape, x.stride()
+    if width < 1:
         raise DiffGraphHipError(f"{name}: rows have no columns")
-    if x.shape[1] > 1 and x.stride(1) != 1 or x.stride(0) < 0:
+    if width > 1 and step != 1 or pitch < 0:
         raise DiffGraphHipError(f"{name}: the elements of a row must lie next to each other (strides {tuple(x.stride())})")
-    if max(x.shape) > 0x7fffffff:
+    if n > 0x7fffffff or width > 0x7fffffff:
         raise DiffGraphHipError(f"{name}: at most 2^31 - 1 rows and columns, got {tuple(x.shape)}")
-    return x
+    return n, width, pitch, _ELEMENT[x.dtype]
 
 
-def _ids(ids: torch.Tensor, device) -> torch.Tensor:
-    if not isinstance(ids, torch.Tensor) or ids.dtype not in (torch.int64, torch.int32) or ids.device != device:
+def _ids(ids: torch.Tensor, at: int):
+    """(contiguous ids, whether they are int64) of a tensor of ids on GPU `at`."""
+    wide = isinstance(ids, torch.Tensor) and ids.dtype == torch.int64
+    if not wide and not (isinstance(ids, torch.Tensor) and ids.dtype == torch.int32) or not ids.is_cuda or ids.get_device() != at:
         raise DiffGraphHipError("ids: expected an int64 or int32 tensor on the table's GPU")
-    return ids if ids.is_contiguous() else ids.contiguous()
+    return ids if ids.is_contiguous() else ids.contiguous(), wide
 
 
 def embedding_lookup(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
     """scale * table[ids] for table [rows, width] (float32 / bfloat16 / float16; rows may lie further apart than their
     width) and int64 / int32 ids of any shape; [*ids.shape, width], rounded once.  An id outside the table: a row of NaN.
     Not recorded by autograd: layers.embedding is."""
-    _rows(table, "table")
-    ids = _ids(ids, table.device)
-    n, dim = table.shape
+    n, dim, pitch, code = _rows(table, "table")
+    at = table.get_device()
+    ids, wide = _ids(ids, at)
     if n < 1:
         raise DiffGraphHipError("table: has no rows to look up")
-    dev = table.device
-    out = torch.empty((*ids.shape, dim), dtype=table.dtype, device=dev)
+    out = table.new_empty((*ids.shape, dim))
     count = ids.numel()
     if count:
-        _lib.launch(dev, _lib.load().dg_embedding_lookup, "dg_embedding_lookup", table.data_ptr(), n, table.stride(0), dim,
-                    _ELEMENT[table.dtype], ids.data_ptr(), ids.dtype == torch.int64, count, scale, out.data_ptr())
+        _lib.launch(at, _lib.load().dg_embedding_lookup, "dg_embedding_lookup", table.data_ptr(), n, pitch, dim, code, ids.data_ptr(), wide,
+                    count, scale, out.data_ptr())
     return out
 
 
@@ -1030,38 +1033,39 @@ def embedding_grad(d_out: torch.Tensor, ids: torch.Tensor, n_rows: int, scale: f
         raise DiffGraphHipError("d_out: expected a tensor of shape [*ids.shape, width], ids a tensor")
     if n_rows < 1:
         raise DiffGraphHipError("n_rows: a table has at least one row")
-    dim, dev = d_out.shape[-1], d_out.device
+    dim = d_out.shape[-1]
     d = d_out if d_out.dim() == 2 else d_out.reshape(-1, dim) if dim else d_out.reshape(0, 0)
     if d.stride(1) != 1 or d.stride(0) < dim and d.shape[0] > 1:
         d = d.contiguous()
-    _rows(d, "d_out")
-    ids = _ids(ids, dev)
+    _, _, pitch, code = _rows(d, "d_out")
+    at = d.get_device()
+    ids, wide = _ids(ids, at)
     if padding_idx is not None and not 0 <= padding_idx < n_rows:
         raise DiffGraphHipError(f"padding_idx must lie in [0,{n_rows}); got {padding_idx}")
     lib, n = _lib.load(), ids.numel()
-    grad = torch.empty((n_rows, dim), dtype=d.dtype, device=dev)
+    grad = d.new_empty((n_rows, dim))
     ws_bytes = lib.dg_embedding_grad_workspace(n, n_rows, dim) if n else 0
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-    _lib.launch(dev, lib.dg_embedding_grad, "dg_embedding_grad", d.data_ptr(), d.stride(0), ids.data_ptr(), ids.dtype == torch.int64, n,
-                n_rows, dim, _ELEMENT[d.dtype], scale, -1 if padding_idx is None else padding_idx, grad.data_ptr(), ws.data_ptr(), ws_bytes)
+    ws = d.new_empty(ws_bytes, dtype=torch.uint8)
+    _lib.launch(at, lib.dg_embedding_grad, "dg_embedding_grad", d.data_ptr(), pitch, ids.data_ptr(), wide, n, n_rows, dim, code, scale,
+                -1 if padding_idx is None else padding_idx, grad.data_ptr(), ws.data_ptr(), ws_bytes)
     return grad
 
 
 # --------------------------------------------------------------------------------------
 # scores
 # --------------------------------------------------------------------------------------
-def _on(x: torch.Tensor, name: str, dtype, device, dims) -> torch.Tensor:
-    if not isinstance(x, torch.Tensor) or x.dtype != dtype or x.device != device or x.dim() not in dims:
-        raise DiffGraphHipError(f"{name}: expected a {' or '.join(f'{d}-D' for d in dims)} {dtype} tensor on {device}")
+def _on(x: torch.Tensor, name: str, dtype, at: int, dims) -> torch.Tensor:
+    if not isinstance(x, torch.Tensor) or x.dtype != dtype or not x.is_cuda or x.get_device() != at or x.dim() not in dims:
+        raise DiffGraphHipError(f"{name}: expected a {' or '.join(f'{d}-D' for d in dims)} {dtype} tensor on cuda:{at}")
     return x
 
 
-def _per_row(v, name: str, n: int, device, neutral: float):
+def _per_row(v, name: str, n: int, at: int, neutral: float):
     """(tensor or None, value for all rows) of a penalty given as a number, a float32 [n] tensor or None."""
     if v is None:
         return None, neutral
     if isinstance(v, torch.Tensor):
-        _on(v, name, torch.float32, device, (1,))
+        _on(v, name, torch.float32, at, (1,))
         if v.numel() != n:
             raise DiffGraphHipError(f"{name}: expected one value for each of {n} rows, got {v.numel()}")
         return v.contiguous(), neutral
@@ -1085,32 +1089,31 @@ def adjust_scores(scores: torch.Tensor, *, history=None, rows: Optional[torch.Te
     row whose number is not that of a mask has none; default: mask r for row r).  A row whose mask leaves nothing is all
     `fill`.  out: where to (scores itself: in place).  Not recorded by autograd, so neither scores nor bias may ask for a gradient
     where one is recorded."""
-    _rows(scores, "scores")
+    n, items, pitch, code = _rows(scores, "scores")
     if torch.is_grad_enabled() and (scores.requires_grad or bias is not None and bias.requires_grad):
         raise DiffGraphHipError("scores, bias: adjust_scores is not recorded by autograd: detach them")
-    n, items = scores.shape
-    dev = scores.device
+    at = scores.get_device()
     if out is None:
-        out = torch.empty((n, items), dtype=scores.dtype, device=dev)
+        out, out_pitch = scores.new_empty((n, items)), items
     else:
-        _rows(out, "out")
-        if out.dtype != scores.dtype or out.shape != scores.shape or out.device != dev:
+        *form, out_pitch, out_code = _rows(out, "out")
+        if out_code != code or form != [n, items] or out.get_device() != at:
             raise DiffGraphHipError("out: expected a tensor of scores' type, shape and device")
         same = out.data_ptr() == scores.data_ptr() and out.stride() == scores.stride()
         if not same and out.untyped_storage().data_ptr() == scores.untyped_storage().data_ptr():
             raise DiffGraphHipError("out: must be scores itself or memory of its own")
-        if n > 1 and out.stride(0) < items:
+        if n > 1 and out_pitch < items:
             raise DiffGraphHipError("out: its rows overlap")
     t = _lib.ScoreTask()
-    t.scores, t.out, t.row_stride, t.out_stride = scores.data_ptr(), out.data_ptr(), scores.stride(0), out.stride(0)
-    t.n_rows, t.n_items, t.dtype, t.exclude, t.fill = n, items, _ELEMENT[scores.dtype], int(bool(exclude)), float(fill)
+    t.scores, t.out, t.row_stride, t.out_stride = scores.data_ptr(), out.data_ptr(), pitch, out_pitch
+    t.n_rows, t.n_items, t.dtype, t.exclude, t.fill = n, items, code, bool(exclude), float(fill)
     if history is not None:
-        rowptr, col = (_on(v, "history", torch.int32, dev, (1,)).contiguous() for v in history)
+        rowptr, col = (_on(v, "history", torch.int32, at, (1,)).contiguous() for v in history)
         if rowptr.numel() < 1:
             raise DiffGraphHipError("history: rowptr has one entry more than there are lines")
         t.n_hist, t.n_hist_items = rowptr.numel() - 1, col.numel()
         if rows is not None:
-            rows = _on(rows, "rows", torch.int64, dev, (1,)).contiguous()
+            rows = _on(rows, "rows", torch.int64, at, (1,)).contiguous()
             if rows.numel() != n:
                 raise DiffGraphHipError(f"rows: expected one entry for each of {n} rows, got {rows.numel()}")
             t.hist_rows = rows.data_ptr()
@@ -1122,26 +1125,26 @@ def adjust_scores(scores: torch.Tensor, *, history=None, rows: Optional[torch.Te
             t.hist_rows = None
     elif rows is not None or exclude or repetition is not None or frequency is not None or presence is not None:
         raise DiffGraphHipError("history: penalties, rows and exclude need one")
-    rep, t.repetition_all = _per_row(repetition, "repetition", n, dev, 1.0)
-    fre, t.frequency_all = _per_row(frequency, "frequency", n, dev, 0.0)
-    pre, t.presence_all = _per_row(presence, "presence", n, dev, 0.0)
+    rep, t.repetition_all = _per_row(repetition, "repetition", n, at, 1.0)
+    fre, t.frequency_all = _per_row(frequency, "frequency", n, at, 0.0)
+    pre, t.presence_all = _per_row(presence, "presence", n, at, 0.0)
     if not t.repetition_all > 0:
         raise DiffGraphHipError(f"repetition must be positive, got {t.repetition_all}")
     t.repetition, t.frequency, t.presence = _ptr(rep), _ptr(fre), _ptr(pre)
     if bias is not None:
-        _on(bias, "bias", torch.float32, dev, (1, 2))
+        _on(bias, "bias", torch.float32, at, (1, 2))
         if bias.shape[-1] != items or (bias.dim() == 2 and bias.shape[0] != n):
             raise DiffGraphHipError(f"bias: expected shape [{items}] or [{n}, {items}], got {tuple(bias.shape)}")
         if items > 1 and bias.stride(-1) != 1 or bias.stride(0) < 0:
             bias = bias.contiguous()
         t.bias, t.bias_stride = bias.data_ptr(), bias.stride(0) if bias.dim() == 2 else 0
     if allowed is not None:
-        allowed = _on(allowed, "allowed", torch.int32, dev, (1, 2)).contiguous()
+        allowed = _on(allowed, "allowed", torch.int32, at, (1, 2)).contiguous()
         if allowed.shape[-1] < (items + 31) // 32:
             raise DiffGraphHipError(f"allowed: {(items + 31) // 32} words hold {items} items, got {allowed.shape[-1]}")
         masks = allowed.shape[0] if allowed.dim() == 2 else 1
         if allowed_rows is not None:
-            allowed_rows = _on(allowed_rows, "allowed_rows", torch.int32, dev, (1,)).contiguous()
+            allowed_rows = _on(allowed_rows, "allowed_rows", torch.int32, at, (1,)).contiguous()
             if allowed_rows.numel() != n:
                 raise DiffGraphHipError(f"allowed_rows: expected one entry for each of {n} rows, got {allowed_rows.numel()}")
         elif masks not in (1, n):
@@ -1152,7 +1155,7 @@ def adjust_scores(scores: torch.Tensor, *, history=None, rows: Optional[torch.Te
     elif allowed_rows is not None:
         raise DiffGraphHipError("allowed: allowed_rows needs masks")
     if n and items:
-        _lib.launch(dev, _lib.load().dg_adjust_scores, "dg_adjust_scores", C.byref(t))
+        _lib.launch(at, _lib.load().dg_adjust_scores, "dg_adjust_scores", C.byref(t))
     return out
 
 
@@ -1175,16 +1178,16 @@ class Checkpoint8:
         if dtype not in _ELEMENT:
             raise DiffGraphHipError(f"values: float32, bfloat16 or float16, not {dtype}")
         n, k = self.shape
-        dev = self.data.device
-        self._check("values", n, dev)
-        out = torch.empty((n, k), dtype=dtype, device=dev)
-        _lib.launch(dev, _lib.load().dg_checkpoint8_values, "dg_checkpoint8_values", self.data.data_ptr(), n, k, _FORMATS[self.format],
+        at = self.data.get_device()
+        self._check("values", n, at)
+        out = self.data.new_empty((n, k), dtype=dtype)
+        _lib.launch(at, _lib.load().dg_checkpoint8_values, "dg_checkpoint8_values", self.data.data_ptr(), n, k, _FORMATS[self.format],
                     _ELEMENT[dtype], out.data_ptr())
         return out
 
-    def _check(self, name: str, n: int, device) -> None:
+    def _check(self, name: str, n: int, at: int) -> None:
         d, k = self.data, self.shape[1]
-        if not d.is_cuda or d.device != device or d.dtype != torch.uint8 or d.numel() != _kept_bytes(self.shape[0], k) or not d.is_contiguous() \
+        if not d.is_cuda or d.get_device() != at or d.dtype != torch.uint8 or d.numel() != _kept_bytes(self.shape[0], k) or not d.is_contiguous() \
                 or self.format not in _FORMATS:
             raise DiffGraphHipError(f"{name}: not what checkpoint8 keeps, or on another device")
         if self.shape[0] != n:
@@ -1198,13 +1201,11 @@ def _kept_bytes(n: int, k: int) -> int:
 def checkpoint8(x: torch.Tensor, format: str = "int8") -> Checkpoint8:
     """x [n, k] (float32 / bfloat16 / float16) in 8 bits: codes of `format` "int8" or "e4m3" and, per 32 columns of a row,
     the smallest power of two that keeps the group's largest within them; each value to the nearest code (ties to even)."""
-    _rows(x, "x")
+    n, k, pitch, code = _rows(x, "x")
     if format not in _FORMATS:
         raise DiffGraphHipError(f"format: 'int8' or 'e4m3', got {format!r}")
-    n, k = x.shape
-    dev = x.device
-    data = torch.empty(_kept_bytes(n, k), dtype=torch.uint8, device=dev)
-    _lib.launch(dev, _lib.load().dg_checkpoint8, "dg_checkpoint8", x.data_ptr(), x.stride(0), n, k, _ELEMENT[x.dtype], _FORMATS[format],
+    data = x.new_empty(_kept_bytes(n, k), dtype=torch.uint8)
+    _lib.launch(x.get_device(), _lib.load().dg_checkpoint8, "dg_checkpoint8", x.data_ptr(), pitch, n, k, code, _FORMATS[format],
                 data.data_ptr())
     return Checkpoint8(data, (n, k), format)
 
@@ -1213,25 +1214,25 @@ def checkpoint8_backward(d_y: torch.Tensor, x: Checkpoint8, y: Optional[Checkpoi
     """(d_z [n, m], d_w [m, k], d_b [m]), of d_y's type, of a dense layer z = x . w^T + b from the gradient d_y [n, m] and
     what was kept of its input x [n, k]: d_w = d_z^T . x, d_b = column sums of d_z, where d_z is d_y (returned as it is), or,
     with what was kept of y = tanh(z), d_y (1 - y y).  Sums in fp32 in a fixed order."""
-    _rows(d_y, "d_y")
-    n, m = d_y.shape
-    dev = d_y.device
+    n, m, pitch, code = _rows(d_y, "d_y")
+    at = d_y.get_device()
     if not isinstance(x, Checkpoint8) or not (y is None or isinstance(y, Checkpoint8)):
         raise DiffGraphHipError("x, y: expected what checkpoint8 returns")
-    x._check("x", n, dev)
+    x._check("x", n, at)
     k = x.shape[1]
     if y is not None:
-        y._check("y", n, dev)
+        y._check("y", n, at)
         if y.shape[1] != m or y.format != x.format:
             raise DiffGraphHipError(f"y: expected {m} columns in the format of x ({x.format})")
     lib = _lib.load()
-    src = d_y if n < 2 or m <= d_y.stride(0) <= 1 << 24 else d_y.contiguous()      # (as the kernel's rows may lie)
+    if n < 2 or not m <= pitch <= 1 << 24:                                          # (as the kernel's rows may lie)
+        pitch = m
+    src = d_y if n < 2 or pitch == d_y.stride(0) else d_y.contiguous()
     ws_bytes = lib.dg_checkpoint8_backward_workspace(n, k, m)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-    d_z = d_y if y is None else torch.empty((n, m), dtype=d_y.dtype, device=dev)
-    d_w = torch.empty((m, k), dtype=d_y.dtype, device=dev)
-    d_b = torch.empty(m, dtype=d_y.dtype, device=dev)
-    _lib.launch(dev, lib.dg_checkpoint8_backward, "dg_checkpoint8_backward", src.data_ptr(), src.stride(0) if n > 1 else m, n, m, k,
-                _ELEMENT[d_y.dtype], _FORMATS[x.format], x.data.data_ptr(), None if y is None else y.data.data_ptr(), d_z.data_ptr(),
-                d_w.data_ptr(), d_b.data_ptr(), ws.data_ptr(), ws_bytes)
+    ws = d_y.new_empty(ws_bytes, dtype=torch.uint8)
+    d_z = d_y if y is None else d_y.new_empty((n, m))
+    d_w, d_b = d_y.new_empty((m, k)), d_y.new_empty(m)
+    _lib.launch(at, lib.dg_checkpoint8_backward, "dg_checkpoint8_backward", src.data_ptr(), pitch, n, m, k, code, _FORMATS[x.format],
+                x.data.data_ptr(), None if y is None else y.data.data_ptr(), d_z.data_ptr(), d_w.data_ptr(), d_b.data_ptr(), ws.data_ptr(),
+                ws_bytes)
     return d_z, d_w, d_b
