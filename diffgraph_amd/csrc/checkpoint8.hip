@@ -480,8 +480,11 @@ row_grid rows_of(int64_t n, int k, int columns) {
   return g;
 }
 
-// Tiles of 128 columns, or 64 where that leaves fewer of them empty; strips so that some 512 workgroups run, two a CU, of
-// some 128 rows at least each (1024: 1e6 rows, 128 -> 64, fp32, tanh 153 against 141 us, for the partial sums they add).
+// Tiles of 128 columns, or 64 where that leaves fewer of them empty; strips so that at most 512 workgroups run, two a CU and
+// all at once (one more than 512, 63114 rows, 136 -> 128, fp32, tanh: 47 against 36 us; 1024, 1e6 rows, 128 -> 64: 153 against
+// 141, for the partial sums they add), of at least 128 rows each (64 rows, 8192 x 256 x 256: 29 against 26 us), and 256 with
+// the largest tile, whose partial sums cost the most (8192 rows, 200 -> 128, bf16: 12.8 us against 16.3 with 128; 512 x 1024 x
+// 1024: 16.3 against 19.7).
 int side_of(int columns) { return (columns + 127) / 128 * 2 > (columns + 63) / 64 ? 64 : 128; }
 struct back_plan {
   int bm, bn, tiles_m, tiles_n, strips;
@@ -494,8 +497,9 @@ back_plan plan_of(int64_t n, int k, int m) {
   p.tiles_m = (m + p.bm - 1) / p.bm;
   p.tiles_n = (k + p.bn - 1) / p.bn;
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
-  int64_t strips = (512 + tiles - 1) / tiles;
-  strips = strips < (n + 127) / 128 ? strips : (n + 127) / 128;
+  const int64_t least = p.bm * p.bn == 128 * 128 ? 256 : 128, most = (n + least - 1) / least;
+  int64_t strips = tiles < 512 ? 512 / tiles : 1;
+  strips = strips < most ? strips : most;
   p.strips = (int)strips;
   p.part = 0;
   p.part_b = (size_t)p.strips * tiles * p.bm * p.bn * 4;
