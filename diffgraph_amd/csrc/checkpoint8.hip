@@ -13,9 +13,9 @@
 // and, with tanh, of its output y:
 //   d_z = d_y (1 - y^ y^)      d_w = d_z^T . x^      d_b = column sums of d_z
 // The product runs on the bf16 matrix instruction: x^ is exact there, and d_z (fp32) is cut into bf16 numbers that add up
-// to it -- three for fp32 (all 24 bits), two for fp16 and for d_z formed from bf16 (16 bits, beyond what the 16-bit result
-// shows), one for bf16 as it came -- with sums in fp32.  Rows are cut into strips whose partial results a second launch
-// adds in strip order: the same bits on every run.
+// to it bit by bit -- three where d_z has 24 bits (fp32, and every type under tanh), two for fp16 as it came (11 bits), one
+// for bf16 as it came -- with sums in fp32.  Rows are cut into strips whose partial results a second launch adds in strip
+// order: the same bits on every run.
 #include "dg_internal.h"
 #include "dg_types.h"
 
@@ -536,11 +536,12 @@ int back_tiles(const back_plan &p, const back_args &a, void *d_w, void *d_b, hip
   return back_as<T, FMT, TANH, PIECES, 64, 64, false>(p, a, (T *)d_w, (T *)d_b, stream);
 }
 
-template <typename T, int PLAIN, int WITH_TANH>
+// PLAIN: the bf16 numbers that hold a value of T; three hold an fp32 value, as d_z is under tanh whatever the type.
+template <typename T, int PLAIN>
 int back_forms(int fmt, bool tanh, const back_plan &p, const back_args &a, void *d_w, void *d_b, hipStream_t stream) {
   if (fmt == DG_E4M3)
-    return tanh ? back_tiles<T, DG_E4M3, true, WITH_TANH>(p, a, d_w, d_b, stream) : back_tiles<T, DG_E4M3, false, PLAIN>(p, a, d_w, d_b, stream);
-  return tanh ? back_tiles<T, DG_INT8, true, WITH_TANH>(p, a, d_w, d_b, stream) : back_tiles<T, DG_INT8, false, PLAIN>(p, a, d_w, d_b, stream);
+    return tanh ? back_tiles<T, DG_E4M3, true, 3>(p, a, d_w, d_b, stream) : back_tiles<T, DG_E4M3, false, PLAIN>(p, a, d_w, d_b, stream);
+  return tanh ? back_tiles<T, DG_INT8, true, 3>(p, a, d_w, d_b, stream) : back_tiles<T, DG_INT8, false, PLAIN>(p, a, d_w, d_b, stream);
 }
 
 }  // namespace
@@ -626,7 +627,7 @@ extern "C" int dg_checkpoint8_backward(const void *d_y, int64_t row_stride, int6
                  pitch_of(k), groups_of(k), pitch_of(m), groups_of(m), n, k, m, p.strips, p.tiles_m, p.tiles_n, d_z,
                  (float *)workspace, (float *)((char *)workspace + p.part_b)};
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == DG_F32) return back_forms<float, 3, 3>(format, tanh, p, a, d_w, d_b, st);
-  if (dtype == DG_BF16) return back_forms<dg_bf16, 1, 2>(format, tanh, p, a, d_w, d_b, st);
-  return back_forms<dg_f16, 2, 2>(format, tanh, p, a, d_w, d_b, st);
+  if (dtype == DG_F32) return back_forms<float, 3>(format, tanh, p, a, d_w, d_b, st);
+  if (dtype == DG_BF16) return back_forms<dg_bf16, 1>(format, tanh, p, a, d_w, d_b, st);
+  return back_forms<dg_f16, 2>(format, tanh, p, a, d_w, d_b, st);
 }

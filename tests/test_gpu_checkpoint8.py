@@ -161,6 +161,28 @@ def test_every_bit_of_an_fp32_gradient_reaches_the_product():
 
 @gpu
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_every_bit_of_d_z_under_tanh_reaches_the_product(dtype, fmt):
+    """Pairs of rows with x = 1 and -1, the same d_y and different y = c 2^-9, |c| <= 15 (codes of either format): an element
+    of d_w is the difference of two d_z that agree in their leading bits, exact in fp32 whatever the order of its pieces'
+    sums (each is a multiple of the smaller one's last place and no larger than d_z), and rounded once to the type."""
+    pairs, m = 32, 70
+    g = torch.Generator().manual_seed(11)
+    d = torch.randn(pairs, 1, m, generator=g).to(dtype).expand(pairs, 2, m).reshape(2 * pairs, m)
+    y = torch.randint(-15, 16, (2 * pairs, m), generator=g).float() * 2.0 ** -9
+    x = torch.zeros(2 * pairs, pairs)
+    x[torch.arange(2 * pairs), torch.arange(2 * pairs) // 2] = torch.tensor([1.0, -1.0]).repeat(pairs)
+    xk, yk = ops.checkpoint8(x.to(dtype).to(DEV), fmt), ops.checkpoint8(y.to(dtype).to(DEV), fmt)
+    assert torch.equal(yk.values().cpu(), y)
+    _, d_w, _ = ops.checkpoint8_backward(d.to(DEV), xk, yk)
+    z = (d.float() * (1 - y * y)).double()                      # (fp32, as the definition of d_z is held)
+    want = (z[0::2] - z[1::2]).t()
+    assert torch.equal(want.float().double(), want) and bool((want != 0).any())
+    assert torch.equal(d_w.cpu(), want.float().to(dtype))
+
+
+@gpu
+@pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("tanh", [False, True], ids=["linear", "tanh"])
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("n,m,k", [(40, 64, 72), (515, 130, 260), (2049, 32, 128), (9000, 100, 50)])
