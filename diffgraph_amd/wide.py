@@ -16,7 +16,7 @@ import torch
 import torch.nn.functional as F
 
 from . import ops
-from ._lib import DG_D
+from ._lib import DG_D, DiffGraphHipError
 from .layers import embedding
 
 
@@ -78,9 +78,12 @@ def cal_loss(model, ancs, poss, negs, ts_u=None, noise_u=None, ts_i=None, noise_
 def all_rank_topk(usr: torch.Tensor, itm: torch.Tensor, users: torch.Tensor, trn_rowptr: torch.Tensor, trn_col: torch.Tensor,
                   topk: int, batch: int = 1024):
     """t.topk(t.mm(usr[users], itm^T) * (1 - trnMask) - trnMask * 1e8, topk) (main.py:157-158) in batches of users,
-    the training items of a row replaced by -1e8 in one pass.  Returns (values [len(users), topk], item ids int32)."""
+    the training items of a row replaced by -1e8 in one pass.  A user outside the tables is refused.  Returns (values [len(users), topk], item ids int32)."""
     n_item = itm.shape[0]
     usr, itm, users = usr.detach(), itm.detach(), users.long().to(usr.device)
+    n_user = min(usr.shape[0], trn_rowptr.numel() - 1)
+    if users.numel() and (int(users.min()) < 0 or int(users.max()) >= n_user):
+        raise DiffGraphHipError(f"users must lie in [0,{n_user})")
     usr = usr if usr.stride(1) == 1 else usr.contiguous()
     vals, idx = [], []
     for b in range(0, users.numel(), batch):

@@ -275,3 +275,27 @@ def test_wide_loss_with_rows_named_many_times():
             wide.embedding = old
         grads.append(m.embedding_table.grad.clone())
     assert_rows_close(grads[0], grads[1], rtol=1e-5, what="table gradient")
+
+
+def test_wide_evaluation_refuses_users_that_are_not_there():
+    """As the narrow tables' evaluation does (and torch's index check did): before anything touches the GPU."""
+    from diffgraph_amd import wide
+    usr, itm = torch.zeros(6, 80), torch.zeros(9, 80)
+    rowptr, col = torch.zeros(7, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    for users in ([6], [0, -1], [5, 6, 1], [-7]):
+        with pytest.raises(DiffGraphHipError, match="users must lie in"):
+            wide.all_rank_topk(usr, itm, torch.tensor(users), rowptr, col, 3)
+    with pytest.raises(DiffGraphHipError, match="users must lie in"):      # a user without a line in the interactions
+        wide.all_rank_topk(usr, itm, torch.tensor([5]), rowptr[:6], col, 3)
+
+
+@gpu
+def test_wide_evaluation_refuses_users_that_are_not_there_through_its_entry_point():
+    data, _ = interactions(30, 50)
+    usr, itm = torch.randn(30, 80, device=DEV), torch.randn(50, 80, device=DEV)
+    for users in ([30], [3, -1]):
+        for width in (64, 80):
+            with pytest.raises(DiffGraphHipError, match="users must lie in"):
+                ev.all_rank_topk(usr[:, :width].contiguous(), itm[:, :width].contiguous(), torch.tensor(users, device=DEV), data, 5)
+    val, idx = ev.all_rank_topk(usr, itm, torch.tensor([29, 0], device=DEV), data, 5)
+    assert bool(val.isfinite().all()) and idx.shape == (2, 5)
