@@ -58,6 +58,12 @@ def propagate(graphs: Sequence, e0: torch.Tensor, n_layers: int, slope: float):
     return sums[0][:, :L], het[:, :L]
 
 
+def row_ids(ids: torch.Tensor, rows: torch.Tensor) -> torch.Tensor:
+    """The rows that ids name in a table whose rows are numbered `rows` = 0 .. n - 1, with torch's own rules: a negative id
+    counts from the end, one outside [-n, n) raises (on the GPU by a device assertion, with no synchronisation here)."""
+    return rows[ids.long().to(rows.device)]
+
+
 def cal_loss(model, ancs, poss, negs, ts_u=None, noise_u=None, ts_i=None, noise_i=None, keep_u=None, keep_i=None) -> torch.Tensor:
     """HGDM.cal_loss (Model.py:94-111) as float64[4] = (loss, bprLoss, regLoss, diff_loss)."""
     dp, nu, args = model.diffusion_process, model.n_user, model.args
@@ -65,7 +71,8 @@ def cal_loss(model, ancs, poss, negs, ts_u=None, noise_u=None, ts_i=None, noise_
                         float(model.act.negative_slope))
     rl_u, out_u = dp.training_losses_rows(model.usr_denoiser, ui[:nu], het[:nu], ts_u, noise_u, keep_u)
     rl_i, out_i = dp.training_losses_rows(model.item_denoiser, ui[nu:], het[nu:], ts_i, noise_i, keep_i)
-    ancs, poss, negs = (v.long().to(ui.device) for v in (ancs, poss, negs))
+    rows = torch.arange(max(nu, model.n_item), device=ui.device)
+    ancs, poss, negs = row_ids(ancs, rows[:nu]), row_ids(poss, rows[:model.n_item]), row_ids(negs, rows[:model.n_item])
     diff = rl_u[ancs].mean() + rl_i[poss].mean()
     usr, itm = ui[:nu] + out_u, ui[nu:] + out_i
     a, p, n = embedding(usr, ancs), embedding(itm, poss), embedding(itm, negs)

@@ -299,3 +299,44 @@ def test_wide_evaluation_refuses_users_that_are_not_there_through_its_entry_poin
                 ev.all_rank_topk(usr[:, :width].contiguous(), itm[:, :width].contiguous(), torch.tensor(users, device=DEV), data, 5)
     val, idx = ev.all_rank_topk(usr, itm, torch.tensor([29, 0], device=DEV), data, 5)
     assert bool(val.isfinite().all()) and idx.shape == (2, 5)
+
+
+def wide_model(latdim, batch, **kw):
+    wl = dgdata.rec_workload("tiny")
+    nu, ni = wl.n_user, wl.n_item
+    graphs = [dg.CSRGraph.from_bipartite(u, i, nu, ni) for (u, i) in [wl.target] + wl.behaviours]
+    handler = SimpleNamespace(userNum=nu, itemNum=ni, target_adj=graphs[0], behavior_mats=graphs[1:])
+    torch.manual_seed(1)
+    m = dg.rec.HGDM(handler, SimpleNamespace(**{**vars(DEFAULT_ARGS), "latdim": latdim, "batch": batch, **kw})).eval()
+    draws = (torch.randint(0, 200, (nu,), device=DEV), torch.randn(nu, latdim, device=DEV), torch.randint(0, 200, (ni,), device=DEV),
+             torch.randn(ni, latdim, device=DEV))
+    return m, nu, ni, draws
+
+
+@gpu
+def test_wide_loss_counts_negative_ids_from_the_end():
+    """As torch's indexing does: the loss and its gradient, bit for bit."""
+    from diffgraph_amd import wide
+    m, nu, ni, draws = wide_model(80, 50)
+    ids = [torch.randint(0, hi, (50,), device=DEV) for hi in (nu, ni, ni)]
+    got = []
+    for turned in ([], [0], [1], [2], [0, 1, 2]):
+        m.zero_grad()
+        part = [v - hi if k in turned else v for k, (v, hi) in enumerate(zip(ids, (nu, ni, ni)))]
+        loss = wide.cal_loss(m, *part, *draws)
+        loss[0].backward()
+        got.append((loss.detach().clone(), m.embedding_table.grad.clone()))
+    assert bool(got[0][0].isfinite().all())
+    for loss, grad in got[1:]:
+        assert torch.equal(loss, got[0][0]) and torch.equal(grad, got[0][1])
+
+
+def test_ids_outside_a_table_raise():
+    """(On the GPU by torch's own assertion there, at the next synchronisation.)"""
+    from diffgraph_amd import wide
+    rows = torch.arange(9)
+    assert wide.row_ids(torch.tensor([0, 6, -1, -7]), rows[:7]).tolist() == [0, 6, 6, 0]
+    assert wide.row_ids(torch.tensor([3], dtype=torch.int32), rows[:7]).dtype == torch.int64
+    for bad in (7, -8, 1 << 40):
+        with pytest.raises(IndexError):
+            wide.row_ids(torch.tensor([0, bad]), rows[:7])
