@@ -92,11 +92,15 @@ def all_rank_topk(usr: torch.Tensor, itm: torch.Tensor, users: torch.Tensor, trn
     if users.numel() and (int(users.min()) < 0 or int(users.max()) >= n_user):
         raise DiffGraphHipError(f"users must lie in [0,{n_user})")
     usr = usr if usr.stride(1) == 1 else usr.contiguous()
+    if trn_col.numel() > 0x7fffffff:
+        raise DiffGraphHipError(f"trn_col: at most 2^31 - 1 interactions, got {trn_col.numel()}")
+    history = (trn_rowptr.to(torch.int32) if trn_rowptr.dtype != torch.int32 else trn_rowptr,
+               trn_col.clamp(-1, n_item).to(torch.int32) if trn_col.dtype != torch.int32 else trn_col)   # (in int32, the kernel's)
     vals, idx = [], []
     for b in range(0, users.numel(), batch):
         u = users[b: b + batch]
         preds = torch.mm(ops.embedding_lookup(usr, u), itm.t())
-        ops.adjust_scores(preds, history=(trn_rowptr, trn_col), rows=u, exclude=True, fill=-1e8, out=preds)
+        ops.adjust_scores(preds, history=history, rows=u, exclude=True, fill=-1e8, out=preds)
         v, i = torch.topk(preds, min(topk, n_item))
         vals.append(v)
         idx.append(i.to(torch.int32))

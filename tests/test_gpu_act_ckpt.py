@@ -340,3 +340,21 @@ def test_ids_outside_a_table_raise():
     for bad in (7, -8, 1 << 40):
         with pytest.raises(IndexError):
             wide.row_ids(torch.tensor([0, bad]), rows[:7])
+
+
+def _wide_tables(nu=40, ni=300, width=80, dtype=torch.float32):
+    data, had = interactions(nu, ni)
+    g = torch.Generator().manual_seed(2)
+    return data, had.to(DEV), torch.randn(nu, width, generator=g).to(dtype).to(DEV), torch.randn(ni, width, generator=g).to(dtype).to(DEV)
+
+
+@gpu
+@pytest.mark.parametrize("rowptr_type,col_type", [(torch.int64, torch.int64), (torch.int64, torch.int32), (torch.int32, torch.int64)])
+def test_wide_evaluation_takes_interactions_of_either_width(rowptr_type, col_type):
+    from diffgraph_amd import wide
+    data, had, usr, itm = _wide_tables()
+    users = torch.tensor([0, 39, 7, 7], device=DEV)
+    want = wide.all_rank_topk(usr, itm, users, data.trn_rowptr, data.trn_col, 9)
+    got = wide.all_rank_topk(usr, itm, users, data.trn_rowptr.to(rowptr_type), data.trn_col.to(col_type), 9)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert not bool(had[users[:, None], want[1].long()].any())
