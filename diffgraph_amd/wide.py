@@ -82,26 +82,32 @@ def cal_loss(model, ancs, poss, negs, ts_u=None, noise_u=None, ts_i=None, noise_
     return torch.stack([bpr + reg + diff, bpr.double(), reg.double(), diff])
 
 
+_MASKED = -1e8        # the score of a training item (main.py:157)
+
+
 def all_rank_topk(usr: torch.Tensor, itm: torch.Tensor, users: torch.Tensor, trn_rowptr: torch.Tensor, trn_col: torch.Tensor,
                   topk: int, batch: int = 1024):
     """t.topk(t.mm(usr[users], itm^T) * (1 - trnMask) - trnMask * 1e8, topk) (main.py:157-158) in batches of users,
-    the training items of a row replaced by -1e8 in one pass.  A user outside the tables is refused.  Returns (values [len(users), topk], item ids int32)."""
-    n_item = itm.shape[0]
-    usr, itm, users = usr.detach(), itm.detach(), users.long().to(usr.device)
+    the training items of a row replaced by -1e8 in one pass.  A user outside the tables is refused.  Returns (values
+    [len(users), topk], differentiable in usr and itm, item ids int32)."""
+    n_item, users = itm.shape[0], users.long().to(usr.device)
     n_user = min(usr.shape[0], trn_rowptr.numel() - 1)
     if users.numel() and (int(users.min()) < 0 or int(users.max()) >= n_user):
         raise DiffGraphHipError(f"users must lie in [0,{n_user})")
-    usr = usr if usr.stride(1) == 1 else usr.contiguous()
     if trn_col.numel() > 0x7fffffff:
         raise DiffGraphHipError(f"trn_col: at most 2^31 - 1 interactions, got {trn_col.numel()}")
     history = (trn_rowptr.to(torch.int32) if trn_rowptr.dtype != torch.int32 else trn_rowptr,
                trn_col.clamp(-1, n_item).to(torch.int32) if trn_col.dtype != torch.int32 else trn_col)   # (in int32, the kernel's)
+    recorded = torch.is_grad_enabled() and (usr.requires_grad or itm.requires_grad)
+    usr = usr if usr.stride(1) == 1 else usr.contiguous()
     vals, idx = [], []
     for b in range(0, users.numel(), batch):
         u = users[b: b + batch]
-        preds = torch.mm(ops.embedding_lookup(usr, u), itm.t())
-        ops.adjust_scores(preds, history=history, rows=u, exclude=True, fill=-1e8, out=preds)
-        v, i = torch.topk(preds, min(topk, n_item))
+        preds = torch.mm(embedding(usr, u) if recorded else ops.embedding_lookup(usr, u), itm.t())
+        scores = preds.detach()
+        scores = ops.adjust_scores(scores, history=history, rows=u, exclude=True, fill=_MASKED, out=None if recorded else scores)
+        if recorded:                        # the same values as elements of the product; a masked one is a constant
+            v = torch.where(v == torch.full_like(v, _MASKED), v, preds.gather(1, i))
         vals.append(v)
         idx.append(i.to(torch.int32))
     return torch.cat(vals), torch.cat(idx)

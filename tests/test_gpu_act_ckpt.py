@@ -358,3 +358,34 @@ def test_wide_evaluation_takes_interactions_of_either_width(rowptr_type, col_typ
     got = wide.all_rank_topk(usr, itm, users, data.trn_rowptr.to(rowptr_type), data.trn_col.to(col_type), 9)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     assert not bool(had[users[:, None], want[1].long()].any())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_wide_evaluation_passes_gradients_to_its_tables(dtype):
+    """The values are scores of the tables, and differentiable in them as torch's mm, mask and topk are: d usr[u] = sum of
+    d value * itm[item], nothing through a masked place; with gradients off the same values and items."""
+    from diffgraph_amd import wide
+    data, had, usr, itm = _wide_tables(dtype=dtype)
+    users, k = torch.tensor([0, 39, 7, 7], device=DEV), 295                  # more than some rows have left
+    with torch.no_grad():
+        plain = wide.all_rank_topk(usr, itm, users, data.trn_rowptr, data.trn_col, k, batch=3)
+    usr.requires_grad_(), itm.requires_grad_()
+    val, idx = wide.all_rank_topk(usr, itm, users, data.trn_rowptr, data.trn_col, k, batch=3)
+    assert val.dtype == dtype and torch.equal(val, plain[0]) and torch.equal(idx, plain[1])
+    masked = had[users[:, None], idx.long()]
+    assert bool(masked.any()) and torch.equal(masked, val.double() < -1e7)
+    d = torch.randn(val.shape, device=DEV).to(dtype)
+    val.backward(d)
+    c = torch.zeros(4, 300, dtype=torch.float64, device=DEV).scatter_(1, idx.long(), d.double().masked_fill(masked, 0))
+    du = torch.zeros(40, 80, dtype=torch.float64, device=DEV).index_add_(0, users, c @ itm.detach().double())
+    di = c.t().contiguous() @ usr.detach().double()[users]
+    # sums of at most 300 products (and two lookups of one row): each rounding a half step of a partial sum, the rows' sums and
+    # the results rounded to the type
+    eps = torch.finfo(dtype).eps
+    size_u = torch.zeros_like(du).index_add_(0, users, c.abs() @ itm.detach().double().abs())
+    size_i = c.abs().t().contiguous() @ usr.detach().double()[users].abs()
+    half = max(2.0 ** -24, eps / 2) if dtype != torch.float64 else eps / 2
+    for got, want, size in ((usr.grad, du, size_u), (itm.grad, di, size_i)):
+        assert got.dtype == dtype
+        assert bool(((got.double() - want).abs() <= (304 * min(half, 2.0 ** -24) * 2 + 4 * half) * size + 1e-30).all())
