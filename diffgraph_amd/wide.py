@@ -103,9 +103,15 @@ def all_rank_topk(usr: torch.Tensor, itm: torch.Tensor, users: torch.Tensor, trn
     vals, idx = [], []
     for b in range(0, users.numel(), batch):
         u = users[b: b + batch]
-        preds = torch.mm(embedding(usr, u) if recorded else ops.embedding_lookup(usr, u), itm.t())
-        scores = preds.detach()
-        scores = ops.adjust_scores(scores, history=history, rows=u, exclude=True, fill=_MASKED, out=None if recorded else scores)
+        if usr.dtype == torch.float64:      # (wider than the kernels' types: torch's lookup, and a table that says what is masked)
+            preds = torch.mm(usr[u], itm.t())
+            had = ops.adjust_scores(torch.zeros(preds.shape, device=preds.device), history=history, rows=u, exclude=True, fill=1.0)
+            scores = preds.detach().masked_fill(had > 0, _MASKED)
+        else:
+            preds = torch.mm(embedding(usr, u) if recorded else ops.embedding_lookup(usr, u), itm.t())
+            scores = preds.detach()
+            scores = ops.adjust_scores(scores, history=history, rows=u, exclude=True, fill=_MASKED, out=None if recorded else scores)
+        v, i = torch.topk(scores, min(topk, n_item))
         if recorded:                        # the same values as elements of the product; a masked one is a constant
             v = torch.where(v == torch.full_like(v, _MASKED), v, preds.gather(1, i))
         vals.append(v)

@@ -361,7 +361,7 @@ def test_wide_evaluation_takes_interactions_of_either_width(rowptr_type, col_typ
 
 
 @gpu
-@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64, torch.bfloat16], ids=str)
 def test_wide_evaluation_passes_gradients_to_its_tables(dtype):
     """The values are scores of the tables, and differentiable in them as torch's mm, mask and topk are: d usr[u] = sum of
     d value * itm[item], nothing through a masked place; with gradients off the same values and items."""
@@ -389,3 +389,13 @@ def test_wide_evaluation_passes_gradients_to_its_tables(dtype):
     for got, want, size in ((usr.grad, du, size_u), (itm.grad, di, size_i)):
         assert got.dtype == dtype
         assert bool(((got.double() - want).abs() <= (304 * min(half, 2.0 ** -24) * 2 + 4 * half) * size + 1e-30).all())
+
+
+@gpu
+def test_wide_evaluation_out_of_wide_numbers():
+    from diffgraph_amd import wide
+    data, had, usr, itm = _wide_tables(dtype=torch.float64)
+    users = torch.arange(40, device=DEV)
+    val, idx = wide.all_rank_topk(usr, itm, users, data.trn_rowptr, data.trn_col, 6)
+    want = (usr @ itm.t()).masked_fill(had, -1e8).topk(6)
+    assert val.dtype == torch.float64 and torch.equal(val, want.values) and torch.equal(idx.long(), want.indices)
