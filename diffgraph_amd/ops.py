@@ -1092,8 +1092,8 @@ def adjust_scores(scores: torch.Tensor, *, history=None, rows: Optional[torch.Te
     n, items, pitch, code = _rows(scores, "scores")
     if torch.is_grad_enabled() and (scores.requires_grad or bias is not None and bias.requires_grad):
         raise DiffGraphHipError("scores, bias: adjust_scores is not recorded by autograd: detach them")
-    at = scores.get_device()
-    if out is None:
+    at, given = scores.get_device(), out is not None
+    if not given:
         out, out_pitch = scores.new_empty((n, items)), items
     else:
         *form, out_pitch, out_code = _rows(out, "out")
@@ -1156,6 +1156,8 @@ def adjust_scores(scores: torch.Tensor, *, history=None, rows: Optional[torch.Te
         raise DiffGraphHipError("allowed: allowed_rows needs masks")
     if n and items:
         _lib.launch(at, _lib.load().dg_adjust_scores, "dg_adjust_scores", C.byref(t))
+    if given:
+        torch.autograd.graph.increment_version(out)          # (a backward pass that saved it finds it changed)
     return out
 
 

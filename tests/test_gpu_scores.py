@@ -173,6 +173,32 @@ def test_many_rows_and_offsets_past_32_bits():
 
 
 @gpu
+def test_in_place_calls_are_seen_by_autograd():
+    """A tensor that a backward pass still needs: changed by the call, it is refused there, as after torch's own."""
+    bias = torch.ones(64, device=DEV)
+    p = torch.randn(2, 64, device=DEV, requires_grad=True)
+    for write in (lambda q: ops.adjust_scores(q, bias=bias, out=q), lambda q: ops.adjust_scores(torch.zeros_like(q), bias=bias, out=q)):
+        q = p * 1
+        loss = (q * q).sum()
+        before, seen = q._version, q.detach()
+        assert write(seen) is seen and q._version > before
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    q = p * 1
+    loss, before = (q * q).sum(), q._version
+    ops.adjust_scores(q.detach(), bias=bias)                    # reads alone
+    with pytest.raises(DiffGraphHipError, match="own"):
+        ops.adjust_scores(q.detach()[:1], bias=bias, out=q.detach()[1:])
+    assert q._version == before
+    loss.backward()
+    assert torch.equal(p.grad, 2 * p)
+    with torch.inference_mode():
+        s = torch.randn(2, 64, device=DEV)
+        want = s + 1
+        assert torch.equal(ops.adjust_scores(s, bias=bias, out=s), want)
+
+
+@gpu
 def test_on_another_stream_and_in_a_graph():
     g = torch.Generator().manual_seed(8)
     rowptr, col = (v.to(DEV) for v in history(16, 5000, 200, g))
