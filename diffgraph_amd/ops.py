@@ -1087,11 +1087,11 @@ def adjust_scores(scores: torch.Tensor, *, history=None, rows: Optional[torch.Te
     presence: a number or float32 [rows].  bias: float32 [items] or [rows, items].  allowed: int32 words of 32 items, bit
     v % 32 of word v // 32 set where item v stays, [words] for all rows or [masks, words] with allowed_rows (int32 [rows]; a
     row whose number is not that of a mask has none; default: mask r for row r).  A row whose mask leaves nothing is all
-    `fill`.  out: where to (scores itself: in place).  Not recorded by autograd, so neither scores nor bias may ask for a gradient
-    where one is recorded."""
+    `fill`.  out: where to (scores itself: in place).  Not recorded by autograd, so neither scores, bias and penalties nor
+    out may ask for a gradient where one is recorded."""
     n, items, pitch, code = _rows(scores, "scores")
-    if torch.is_grad_enabled() and (scores.requires_grad or bias is not None and bias.requires_grad):
-        raise DiffGraphHipError("scores, bias: adjust_scores is not recorded by autograd: detach them")
+    if torch.is_grad_enabled() and any(isinstance(v, torch.Tensor) and v.requires_grad for v in (scores, bias, repetition, frequency, presence, out)):
+        raise DiffGraphHipError("scores, bias, penalties, out: adjust_scores is not recorded by autograd: detach them")
     at, given = scores.get_device(), out is not None
     if not given:
         out, out_pitch = scores.new_empty((n, items)), items

@@ -282,3 +282,19 @@ def test_tensors_that_ask_for_a_gradient():
         with torch.no_grad():
             assert torch.equal(ops.adjust_scores(scores, bias=bias), scores)
     assert torch.equal(ops.adjust_scores(s.detach(), bias=b.detach()), s.detach())
+
+
+@gpu
+@pytest.mark.parametrize("name", ["repetition", "frequency", "presence", "out"])
+def test_penalties_and_outputs_that_ask_for_a_gradient(name):
+    """A penalty's gradient would be lost as a score's would; an output that asks for one takes no unrecorded values."""
+    s = torch.randn(2, 64, device=DEV)
+    h = (torch.tensor([0, 1, 3], dtype=torch.int32, device=DEV), torch.tensor([5, 7, 7], dtype=torch.int32, device=DEV))
+    asks = torch.ones(2, 64, device=DEV, requires_grad=True) if name == "out" else torch.full((2,), 1.5, device=DEV, requires_grad=True)
+    with pytest.raises(DiffGraphHipError, match="autograd"):
+        ops.adjust_scores(s, history=h, **{name: asks})
+    want = ops.adjust_scores(s, history=h, **({} if name == "out" else {name: asks.detach()}))
+    with torch.no_grad():
+        assert torch.equal(ops.adjust_scores(s, history=h, **{name: asks}), want)
+    with pytest.raises(DiffGraphHipError, match="bias"):
+        ops.adjust_scores(s, bias=[0.0] * 64)
