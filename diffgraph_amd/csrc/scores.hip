@@ -137,15 +137,16 @@ extern "C" int dg_adjust_scores(const dg_score_task *t, void *stream) {
   if (t->hist_rowptr && (t->n_hist < 0 || t->n_hist_items < 0 || (!t->hist_rows && t->n_hist < t->n_rows)))
     return dg_fail(DG_ERR_ARG, "dg_adjust_scores: %lld histories for %d rows", (long long)t->n_hist, t->n_rows);
   if (!t->repetition && !(t->repetition_all > 0.f)) return dg_fail(DG_ERR_ARG, "dg_adjust_scores: the repetition penalty must be positive");
-  if (t->allowed && (t->n_masks < 1 || t->mask_words < ((int64_t)t->n_items + 31) / 32))
-    return dg_fail(DG_ERR_ARG, "dg_adjust_scores: a mask has at least %d words, got %lld", (t->n_items + 31) / 32, (long long)t->mask_words);
+  const int64_t words = ((int64_t)t->n_items + 31) / 32;
+  if (t->allowed && (t->n_masks < 1 || t->mask_words < words))
+    return dg_fail(DG_ERR_ARG, "dg_adjust_scores: a mask has at least %lld words, got %lld", (long long)words, (long long)t->mask_words);
   if (t->allowed && !t->allowed_rows && t->n_masks != 1 && t->n_masks < t->n_rows)
     return dg_fail(DG_ERR_ARG, "dg_adjust_scores: %d masks for %d rows", t->n_masks, t->n_rows);
   if (t->bias && t->bias_stride < 0) return dg_fail(DG_ERR_ARG, "dg_adjust_scores: negative bias stride");
   score_args a = {t->scores, t->out, t->row_stride, t->out_stride, 0, t->n_items, t->hist_rowptr, t->hist_col, t->hist_rows, t->n_hist,
                   t->n_hist_items, t->repetition, t->frequency, t->presence, t->repetition_all, t->frequency_all, t->presence_all, t->bias,
                   t->bias_stride, (const uint8_t *)t->allowed, t->allowed_rows, t->mask_words * 4, t->n_masks, t->exclude, t->fill};
-  const int tiles = (t->n_items + kTile - 1) / kTile;
+  const int tiles = (int)(((int64_t)t->n_items + kTile - 1) / kTile);
   for (int r0 = 0; r0 < t->n_rows; r0 += 65535) {        // (the grid's second axis holds that many)
     const dim3 grid(tiles, t->n_rows - r0 < 65535 ? t->n_rows - r0 : 65535);
     score_args b = a;

@@ -173,6 +173,20 @@ def test_many_rows_and_offsets_past_32_bits():
 
 
 @gpu
+def test_the_longest_row():
+    """2^31 - 1 items: the last tile ends where a 32-bit count of items does."""
+    items = (1 << 31) - 1
+    scores = torch.zeros(1, items, dtype=torch.bfloat16, device=DEV)
+    at = [0, 4095, 4096, items - 4096, items - 4095, items - 1]
+    col = torch.tensor(at + at[-1:], dtype=torch.int32, device=DEV)
+    rowptr = torch.tensor([0, len(at) + 1], dtype=torch.int32, device=DEV)
+    ops.adjust_scores(scores, history=(rowptr, col), frequency=2.0, out=scores)
+    assert scores[0, at].tolist() == [-2.0] * (len(at) - 1) + [-4.0]
+    scores[0, at] = 0
+    assert not bool(scores.any())
+
+
+@gpu
 def test_in_place_calls_are_seen_by_autograd():
     """A tensor that a backward pass still needs: changed by the call, it is refused there, as after torch's own."""
     bias = torch.ones(64, device=DEV)
@@ -298,3 +312,11 @@ def test_penalties_and_outputs_that_ask_for_a_gradient(name):
         assert torch.equal(ops.adjust_scores(s, history=h, **{name: asks}), want)
     with pytest.raises(DiffGraphHipError, match="bias"):
         ops.adjust_scores(s, bias=[0.0] * 64)
+
+
+def test_c_entry_names_the_words_of_the_longest_mask():
+    import ctypes as C
+    items, p = (1 << 31) - 1, 1 << 20
+    t = _lib.ScoreTask(scores=p, out=p, row_stride=items, out_stride=items, n_rows=1, n_items=items, repetition_all=1.0, allowed=p, n_masks=1,
+                       mask_words=(1 << 26) - 1)
+    assert _lib.load().dg_adjust_scores(C.byref(t), None) == -1 and b"at least 67108864 words" in _lib.load().dg_last_error()
