@@ -147,8 +147,8 @@ extern "C" int dg_adjust_scores(const dg_score_task *t, void *stream) {
                   t->n_hist_items, t->repetition, t->frequency, t->presence, t->repetition_all, t->frequency_all, t->presence_all, t->bias,
                   t->bias_stride, (const uint8_t *)t->allowed, t->allowed_rows, t->mask_words * 4, t->n_masks, t->exclude, t->fill};
   const int tiles = (int)(((int64_t)t->n_items + kTile - 1) / kTile);
-  for (int r0 = 0; r0 < t->n_rows; r0 += 65535) {        // (the grid's second axis holds that many)
-    const dim3 grid(tiles, t->n_rows - r0 < 65535 ? t->n_rows - r0 : 65535);
+  for (int64_t r0 = 0; r0 < t->n_rows; r0 += 65535) {    // (the grid's second axis holds that many)
+    const dim3 grid(tiles, (unsigned)(t->n_rows - r0 < 65535 ? t->n_rows - r0 : 65535));
     score_args b = a;
     b.first_row = r0;
     if (t->dtype == DG_F32) hipLaunchKernelGGL((adjust_scores_kernel<float, 4>), grid, dim3(256), 0, (hipStream_t)stream, b);

@@ -187,6 +187,15 @@ def test_the_longest_row():
 
 
 @gpu
+def test_the_most_rows():
+    """2^31 - 1 rows of one item: the launches' first rows end where a 32-bit one would."""
+    n = (1 << 31) - 1
+    scores = torch.zeros(n, 1, dtype=torch.bfloat16, device=DEV)
+    ops.adjust_scores(scores, bias=torch.ones(1, device=DEV), out=scores)
+    assert bool((scores == 1).all())
+
+
+@gpu
 def test_in_place_calls_are_seen_by_autograd():
     """A tensor that a backward pass still needs: changed by the call, it is refused there, as after torch's own."""
     bias = torch.ones(64, device=DEV)
