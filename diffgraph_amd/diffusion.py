@@ -57,6 +57,7 @@ class _Dense8Fn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, kept, w, b, fmt, tanh):
+        ctx.set_materialize_grads(False)          # (autograd would fill a gradient of the codes' size with zeros)
         x, w = x.contiguous(), w.contiguous()
         if kept is None:
             kept = ops.checkpoint8(x, fmt).data
@@ -72,6 +73,8 @@ class _Dense8Fn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, _kept):
+        if dy is None:
+            return (None,) * 6
         w, kept, *y = ctx.saved_tensors
         fmt, x_shape, y_shape = ctx.aux
         y = ops.Checkpoint8(y[0], y_shape, fmt) if y else None

@@ -126,6 +126,65 @@ def test_backward_against_differences(fmt):
         assert abs(float(d_b[o]) - diff) <= abs(float(c[0, o])) * (h * h + 1e-10) + 4 * 2.0 ** -24 * abs(diff) + 1e-10
 
 
+def _on_the_cpu(monkeypatch):
+    """The operators that a dense layer with kept activations calls, by plain stand-ins that keep every bit."""
+    from diffgraph_amd import diffusion
+    kept = {}
+
+    def keep(x, fmt):
+        ck = ops.Checkpoint8(torch.full((x.numel(),), len(kept), dtype=torch.uint8), tuple(x.shape), fmt)
+        kept[len(kept)] = x.detach().clone()
+        return ck
+
+    def backward(d_y, x, y=None):
+        d_z = d_y if y is None else d_y * (1 - kept[int(y.data[0])] ** 2)
+        return d_z, d_z.t() @ kept[int(x.data[0])], d_z.sum(0)
+    monkeypatch.setattr(diffusion.ops, "checkpoint8", keep)
+    monkeypatch.setattr(diffusion.ops, "checkpoint8_backward", backward)
+    monkeypatch.setattr(diffusion.ops, "linear_fwd", lambda x, w, b: torch.nn.functional.linear(x, w, b))
+    return diffusion._Dense8Fn
+
+
+def test_no_gradient_is_made_for_the_codes(monkeypatch):
+    """The codes are a second output of a layer with tanh: its backward pass gets none for them, where autograd would fill a
+    tensor of their size with zeros."""
+    fn = _on_the_cpu(monkeypatch)
+    got, inner = [], fn.backward
+
+    def spy(ctx, dy, codes):
+        got.append((dy is None, codes is None))
+        return inner(ctx, dy, codes)
+    monkeypatch.setattr(fn, "backward", staticmethod(spy))
+    x, w, b = torch.randn(5, 6, requires_grad=True), torch.randn(4, 6, requires_grad=True), torch.randn(4, requires_grad=True)
+    w2, b2 = torch.randn(3, 4, requires_grad=True), torch.randn(3, requires_grad=True)
+    h, kept = fn.apply(x, None, w, b, "int8", True)
+    y, none = fn.apply(h, kept, w2, b2, "int8", False)
+    assert kept.dtype == torch.uint8 and not kept.requires_grad and none is None
+    d = torch.randn_like(y)
+    grads = torch.autograd.grad(y, (x, w, b, w2, b2), d)
+    want = torch.autograd.grad(torch.tanh(x @ w.t() + b) @ w2.t() + b2, (x, w, b, w2, b2), d)
+    for a, c in zip(grads, want):
+        torch.testing.assert_close(a, c)
+    assert got == [(False, True), (False, True)]
+
+
+def test_a_layer_that_no_gradient_reaches(monkeypatch):
+    """Its output goes into a function that passes none on."""
+    class Stop(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, h, x):
+            return h + x
+
+        @staticmethod
+        def backward(ctx, d):
+            return None, d
+    fn = _on_the_cpu(monkeypatch)
+    x, w, b = torch.randn(5, 4, requires_grad=True), torch.randn(4, 4, requires_grad=True), torch.randn(4, requires_grad=True)
+    h, _ = fn.apply(x, None, w, b, "e4m3", True)
+    Stop.apply(h, x).sum().backward()
+    assert torch.equal(x.grad, torch.ones(5, 4)) and (w.grad is None or not bool(w.grad.any()))
+
+
 def test_denoiser_refuses_another_format():
     with pytest.raises(ValueError, match="act_ckpt"):
         dg.Denoise([96, 40], [40, 96], 8, act_ckpt="int4")
