@@ -89,6 +89,8 @@ class Denoise(nn.Module):
     ("int8" / "e4m3"): the layer-by-layer form keeps its activations for the backward pass in 8 bits (the fused kernels
     keep none and take no notice)."""
 
+    act_ckpt = None        # (of modules pickled before there was one)
+
     def __init__(self, in_dims, out_dims, emb_size, norm=False, dropout=0.5, act_ckpt=None):
         super().__init__()
         if act_ckpt not in (None, "int8", "e4m3"):

@@ -126,6 +126,14 @@ def test_backward_against_differences(fmt):
         assert abs(float(d_b[o]) - diff) <= abs(float(c[0, o])) * (h * h + 1e-10) + 4 * 2.0 ** -24 * abs(diff) + 1e-10
 
 
+def test_a_denoiser_pickled_before_it_kept_anything():
+    """A whole pickled module of a version without act_ckpt (as the reference saves its models) keeps nothing in 8 bits."""
+    import pickle
+    d = dg.Denoise([96, 40], [40, 96], 8)
+    del d.__dict__["act_ckpt"]
+    assert pickle.loads(pickle.dumps(d)).act_ckpt is None
+
+
 def _on_the_cpu(monkeypatch):
     """The operators that a dense layer with kept activations calls, by plain stand-ins that keep every bit."""
     from diffgraph_amd import diffusion
