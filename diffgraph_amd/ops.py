@@ -1176,7 +1176,8 @@ class Checkpoint8:
     format: str
 
     def values(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
-        """The [n, k] values the codes stand for (exact in float32 and bfloat16)."""
+        """The [n, k] values the codes stand for (exact in float32 and bfloat16; one that rounds up to a power of two beyond
+        dtype's largest number is an infinity)."""
         if dtype not in _ELEMENT:
             raise DiffGraphHipError(f"values: float32, bfloat16 or float16, not {dtype}")
         n, k = self.shape
@@ -1202,7 +1203,8 @@ def _kept_bytes(n: int, k: int) -> int:
 
 def checkpoint8(x: torch.Tensor, format: str = "int8") -> Checkpoint8:
     """x [n, k] (float32 / bfloat16 / float16) in 8 bits: codes of `format` "int8" or "e4m3" and, per 32 columns of a row,
-    the smallest power of two that keeps the group's largest within them; each value to the nearest code (ties to even)."""
+    the smallest power of two that keeps the group's largest within them; each value to the nearest code (ties to even): off by
+    less than 1/127 of the group's largest in int8, by 2^-4 of the value or 2^-10 of the scale in e4m3.  Not recorded by autograd."""
     n, k, pitch, code = _rows(x, "x")
     if format not in _FORMATS:
         raise DiffGraphHipError(f"format: 'int8' or 'e4m3', got {format!r}")
@@ -1215,7 +1217,9 @@ def checkpoint8(x: torch.Tensor, format: str = "int8") -> Checkpoint8:
 def checkpoint8_backward(d_y: torch.Tensor, x: Checkpoint8, y: Optional[Checkpoint8] = None):
     """(d_z [n, m], d_w [m, k], d_b [m]), of d_y's type, of a dense layer z = x . w^T + b from the gradient d_y [n, m] and
     what was kept of its input x [n, k]: d_w = d_z^T . x, d_b = column sums of d_z, where d_z is d_y (returned as it is), or,
-    with what was kept of y = tanh(z), d_y (1 - y y).  Sums in fp32 in a fixed order."""
+    with what was kept of y = tanh(z), d_y (1 - y y).  Sums in fp32 in a fixed order.  1 - y y is that of the kept y: off by at
+    most 2 |y| Y + Y^2 for a code off by Y (2^-7 in int8, 2^-5 in e4m3, beside a y near 1), and 0 where y is kept as 1 (|y| above
+    1 - 2^-7, 1 - 2^-5): such a unit passes no gradient.  Not recorded by autograd."""
     n, m, pitch, code = _rows(d_y, "d_y")
     at = d_y.get_device()
     if not isinstance(x, Checkpoint8) or not (y is None or isinstance(y, Checkpoint8)):

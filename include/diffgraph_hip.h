@@ -766,7 +766,9 @@ int dg_adjust_scores(const dg_score_task *task, void *stream);
  *                            x [n][k] and, with tanh, of y [n][m] (both in `format`):
  *                              d_z = d_y (1 - y y) (written with tanh only), d_w[m][k] = d_z^T . x, d_b[m] = column sums
  *                            in fp32 over strips of rows added in strip order, every output rounded once to dtype.  A
- *                            column of d_y with an infinity or a NaN in it gives no finite row of d_w
+ *                            column of d_y with an infinity or a NaN in it gives no finite row of d_w.  1 - y y is that of
+ *                            the kept y: off by at most 2 |y| Y + Y^2, Y = the code's error (2^-7 / 2^-5 beside a y near 1),
+ *                            and 0 where y is kept as 1 (|y| > 1 - 2^-7 / 1 - 2^-5)
  * dtype (x, out, d_y, d_z, d_w, d_b): DG_F32 / DG_BF16 / DG_F16; row_stride: elements between the rows of x / d_y (of d_y:
  * m to 2^24).  At most 2^31 - 1 rows of 2^20 columns, 2^35 elements in all.  Kept bytes and workspace: DEVICE, 16-byte
  * aligned.  workspace: dg_checkpoint8_backward_workspace bytes, contents irrelevant; calls that may run at the same time

@@ -75,6 +75,98 @@ def test_denoiser_forward_is_unchanged_and_gradients_follow_the_kept_values(n, f
     assert bool(((last - ref).abs() <= bound).all())
 
 
+def code_error(v, fmt):
+    """How far a code's value may be from v [n, k], by the definition: half a scale in int8, half a step of three bits in
+    e4m3 (below its normal numbers: 2^-10 of the scale).  The scale is at most the power of two above largest / Q."""
+    n, k = v.shape
+    q = 127.0 if fmt == "int8" else 448.0
+    top = torch.nn.functional.pad(v.abs(), (0, -k % 32)).view(n, -1, 32).amax(2)
+    scale = torch.exp2(torch.floor(torch.log2(top.clamp(min=1e-30) / q)) + 1).repeat_interleave(32, 1)[:, :k]
+    return scale / 2 if fmt == "int8" else torch.maximum(v.abs() * 2.0 ** -4, scale * 2.0 ** -10)
+
+
+@gpu
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("n,gain", [(1, 1.0), (77, 1.0), (1500, 1.0), (1, 4.0), (77, 4.0)])
+def test_every_gradient_stays_within_what_the_codes_explain(n, gain, fmt):
+    """The denoiser that keeps 8 bits against the one that keeps everything: inputs, weights and biases of every layer.  With
+    X and Y the errors of the codes of a layer's input x and output y, and E that of the gradient d that reaches it:
+    tanh' = 1 - y^2 is off by T <= 2 |y| Y + Y^2, d_z by Z <= E tanh' + |d| T + E T (Z = E without tanh), d_w by
+    Z^T (|x| + X) + |d_z|^T X, d_b by the column sums of Z, and the layer before gets E = Z |W|.  Beside these, sums of n (or
+    m) products in fp32 in either pass.  gain 4: most units beyond |z| = 2."""
+    U = 2.0 ** -24
+    dn, plain = denoiser(fmt, seed=2), denoiser(None)
+    with torch.no_grad():
+        for layer, tanh in dense_layers(dn):
+            if tanh:
+                layer.weight.mul_(gain)
+    plain.load_state_dict(dn.state_dict())
+    g = torch.Generator().manual_seed(n)
+    x1 = torch.randn(n, 96, generator=g).to(DEV).requires_grad_()
+    x2 = x1.detach().clone().requires_grad_()
+    t, keep = torch.randint(0, 200, (n,), generator=g).to(DEV), (torch.rand(n, 96, generator=g) < 0.5).to(DEV)
+    d_out = torch.randn(n, 96, generator=g).to(DEV)
+    dn(x1, t, True, keep).backward(d_out)
+    plain(x2, t, True, keep).backward(d_out)
+    layers, acts = list(zip(dense_layers(dn), dense_layers(plain))), []
+    with torch.no_grad():
+        e = torch.arange(5, device=DEV, dtype=torch.float32)
+        f = t[:, None].float() * torch.exp(-math.log(10000) * e / 5)[None]
+        emb = ops.linear_fwd(torch.cat([torch.cos(f), torch.sin(f)], 1).contiguous(), dn.emb_layer.weight, dn.emb_layer.bias)
+        h = torch.cat([torch.nn.functional.normalize(x1) * (keep.float() * 2.0), emb], 1)
+        for (layer, tanh), _ in layers:
+            x = h.double()
+            h = ops.linear_fwd(h.contiguous(), layer.weight, layer.bias)
+            h = torch.tanh(h) if tanh else h
+            acts.append((x, h.double()))
+    d, E, saturated, close = d_out.double(), torch.zeros(n, 96, dtype=torch.float64, device=DEV), 0, []
+    for ((layer, tanh), (ref, _)), (x, y) in reversed(list(zip(layers, acts))):
+        X = code_error(x, fmt)
+        if tanh:
+            Y, slope = code_error(y, fmt), 1 - y * y
+            T = 2 * y.abs() * Y + Y * Y
+            Z, d = E * slope + d.abs() * T + E * T + 8 * U * (d.abs() + E), d * slope
+            saturated += int((y.abs() > 1 - 2.0 ** -7).sum())
+        else:
+            Z = E
+        sums = (n + 1000) * 8 * U
+        w_off = Z.t() @ (x.abs() + X) + d.abs().t() @ X + sums * (d.abs() + Z).t() @ (x.abs() + X)
+        b_off = Z.sum(0) + sums * (d.abs() + Z).sum(0)
+        assert bool(((layer.weight.grad.double() - ref.weight.grad.double()).abs() <= w_off).all()), (layer, "d weight")
+        assert bool(((layer.bias.grad.double() - ref.bias.grad.double()).abs() <= b_off).all()), (layer, "d bias")
+        close.append(float((w_off < 0.5 * ref.weight.grad.double().abs()).double().mean()))
+        W = layer.weight.detach().double()
+        E, d = (Z + (layer.weight.shape[0] + 10) * 8 * U * (d.abs() + Z)) @ W.abs(), d @ W
+    # through the kept part of the rows and normalize: (g - u (u . g)) / |x|, u = x / |x|
+    g, g_off = d[:, :96] * keep.double() * 2, E[:, :96] * keep.double() * 2 + 1e-5 * d[:, :96].abs()
+    norm = x1.detach().double().norm(dim=1, keepdim=True)
+    u = x1.detach().double() / norm
+    off = (g_off + u.abs() * (u.abs() * g_off).sum(1, keepdim=True) + 1e-5 * (g.abs() + u.abs() * (u * g).abs().sum(1, keepdim=True))) / norm
+    assert bool(((x1.grad.double() - x2.grad.double()).abs() <= off).all()), "d x"
+    assert bool(x1.grad.any()) and bool(x1.grad.isfinite().all())
+    assert (saturated > 0) == (gain > 1) or n > 1
+    if n == 1 and gain == 1 and fmt == "int8":      # one row, where nothing cancels: the bounds of the last two layers say something
+        assert min(close[:2]) > 0.5, close
+
+
+@gpu
+@pytest.mark.parametrize("fmt,flat", [("int8", 1 - 2.0 ** -7), ("e4m3", 1 - 2.0 ** -5)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+def test_the_slope_of_saturated_units(dtype, fmt, flat):
+    """tanh' out of the codes, beside a unit at 1: within 2 |y| Y + Y^2 of the true one, and exactly 0 where y is kept as 1, from
+    half a step below 1 on; not 0 before."""
+    z = torch.cat([torch.linspace(-6, 6, 31 * 40, dtype=torch.float64).view(40, 31), torch.full((40, 1), 9.0, dtype=torch.float64)], 1)
+    y = torch.tanh(z).to(dtype).to(DEV)
+    x = ops.checkpoint8(torch.ones(40, 3, dtype=dtype, device=DEV), fmt)
+    d_z, _, d_b = ops.checkpoint8_backward(torch.ones(40, 32, dtype=dtype, device=DEV), x, ops.checkpoint8(y, fmt))
+    v = y.double()
+    off = 2.0 ** -7 if fmt == "int8" else torch.maximum(v.abs() * 2.0 ** -4, torch.full_like(v, 2.0 ** -18)).clamp(max=2.0 ** -5)
+    bound = 2 * v.abs() * off + off * off
+    assert bool(((d_z.double() - (1 - v * v)).abs() <= bound + torch.finfo(dtype).eps / 2 + 2.0 ** -23).all())
+    assert not bool(d_z[v.abs() > flat].any()) and bool((d_z[v.abs() < flat] > 0).all())
+    assert bool((d_b > 0).any())
+
+
 @gpu
 def test_kept_bytes():
     """What autograd holds between the passes, apart from the weights: a quarter of the fp32 activations and a little."""
@@ -466,3 +558,37 @@ def test_wide_evaluation_out_of_wide_numbers():
     val, idx = wide.all_rank_topk(usr, itm, users, data.trn_rowptr, data.trn_col, 6)
     want = (usr @ itm.t()).masked_fill(had, -1e8).topk(6)
     assert val.dtype == torch.float64 and torch.equal(val, want.values) and torch.equal(idx.long(), want.indices)
+
+
+@gpu
+def test_recommendations_out_of_trained_tables_are_the_best_that_are_left():
+    """After a training epoch with kept activations and looked-up rows: every returned item's own score is its value, in
+    descending order, no training item is among the finite ones, and nothing better was left out."""
+    from diffgraph_amd.train import Coach
+    from tests.test_gpu_train import _handler
+    args = copy.copy(DEFAULT_ARGS)
+    args.batch, args.dims, args.d_emb_size, args.epoch, args.latdim, args.act_ckpt = 64, "[128, 32]", 10, 1, 128, "int8"
+    torch.manual_seed(8)
+    handler = _handler()
+    c = Coach(handler, args, device=DEV, seed=3)
+    c.prepareModel()
+    c.trainEpoch()
+    with torch.no_grad():
+        usr, itm = c.model.predict()
+    data = handler.tst_data
+    users = data.test_users_dev
+    val, idx = ev.recommend(usr, itm, users, data, 5)
+    v2, i2 = ev.all_rank_topk(usr, itm, users, data, 5)
+    scores = torch.mm(usr[users], itm.t()).double()
+    size = usr.abs().double()[users] @ itm.abs().double().t()
+    off = 2 * (usr.shape[1] + 1) * 2.0 ** -24 * size.max()          # products of other shapes may add in another order
+    ptr, col = data.trn_rowptr.cpu().tolist(), data.trn_col.cpu().tolist()
+    for r, u in enumerate(users.tolist()):
+        had = set(col[ptr[u]: ptr[u + 1]])
+        left = torch.tensor([i for i in range(data.n_item) if i not in had], device=DEV)
+        for v, i, out in ((val[r], idx[r], -math.inf), (v2[r], i2[r], -1e8)):
+            items, n = i.tolist(), min(5, left.numel())
+            assert len(set(items)) == 5 and not any(k in had for k in items[:n]) and bool((v[n:] == out).all())
+            best = scores[r, left].topk(n).values
+            assert bool(((scores[r, i[:n].long()] - v[:n].double()).abs() <= off).all()) and bool(((best - v[:n].double()).abs() <= off).all())
+            assert bool((v[1:n] <= v[:n - 1]).all()) if n > 1 else True
