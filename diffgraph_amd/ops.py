@@ -1090,8 +1090,6 @@ def adjust_scores(scores: torch.Tensor, *, history=None, rows: Optional[torch.Te
     `fill`.  out: where to (scores itself: in place).  Not recorded by autograd, so neither scores, bias and penalties nor
     out may ask for a gradient where one is recorded."""
     n, items, pitch, code = _rows(scores, "scores")
-    if torch.is_grad_enabled() and any(isinstance(v, torch.Tensor) and v.requires_grad for v in (scores, bias, repetition, frequency, presence, out)):
-        raise DiffGraphHipError("scores, bias, penalties, out: adjust_scores is not recorded by autograd: detach them")
     at, given = scores.get_device(), out is not None
     if not given:
         out, out_pitch = scores.new_empty((n, items)), items
@@ -1154,6 +1152,10 @@ def adjust_scores(scores: torch.Tensor, *, history=None, rows: Optional[torch.Te
         t.allowed, t.allowed_rows, t.mask_words, t.n_masks = allowed.data_ptr(), _ptr(allowed_rows), allowed.shape[-1], masks
     elif allowed_rows is not None:
         raise DiffGraphHipError("allowed: allowed_rows needs masks")
+    if torch.is_grad_enabled():
+        for v in (scores, bias, rep, fre, pre, out):
+            if v is not None and v.requires_grad:
+                raise DiffGraphHipError("scores, bias, penalties, out: adjust_scores is not recorded by autograd: detach them")
     if n and items:
         _lib.launch(at, _lib.load().dg_adjust_scores, "dg_adjust_scores", C.byref(t))
     if given:
