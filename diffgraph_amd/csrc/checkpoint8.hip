@@ -124,7 +124,8 @@ __global__ __launch_bounds__(256) void checkpoint8_kernel(const T *__restrict__ 
   }
 }
 
-// The same the other way round, four columns a lane: bound by memory (4097 x 333 fp16 in 3.4 us, mostly a launch's latency).
+// The same the other way round, four columns a lane: bound by memory (1e6 rows of 128 to fp32: 5.9 TB/s; 4097 x 333
+// fp16 in 3.4 us, mostly a launch's latency).
 template <typename T, int FMT>
 __global__ __launch_bounds__(256) void checkpoint8_values_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales,
                                                                  int64_t n, int k, int pitch, int lanes, int quads_per_block,
@@ -204,9 +205,9 @@ struct back_regs {
 // the next step runs beside the matrix instructions of this one.  A block's rows end with their descriptors: rows behind
 // the last one, and whole blocks behind it, come as zeros, with no branch round a load.
 // Bound by memory for few columns (1e6 rows, 128 -> 64, fp32, tanh: 710 MB in 135 us, 5.3 TB/s), for many by conversion,
-// LDS and matrix instructions that overlap in part (16384 rows, 1000 -> 1000, bf16: 58 us, 565 TFLOP/s; some 24, 20 and 14
-// us of vector, LDS and matrix cycles on a SIMD).  Paths of their own for odd widths and for the tiles that form no column
-// sums: 57 us, not kept.
+// LDS and matrix instructions that overlap in part (16384 rows, 1000 -> 1000, bf16, with the strips' sums: 58 us, 565 TFLOP/s;
+// some 24, 20 and 14 us of vector, LDS and matrix cycles on a SIMD; under tanh, three bf16 numbers a d_z: 140 us).  Paths of
+// their own for odd widths and for the tiles that form no column sums: 57 us, not kept.
 // NARROW: d_y has one column (a load of two would leave its row).
 template <typename T, int FMT, bool TANH, int PIECES, int BM, int BN, bool NARROW>
 __global__ __launch_bounds__(256) void checkpoint8_backward_kernel(back_args a) {

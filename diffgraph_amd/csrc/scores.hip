@@ -9,7 +9,7 @@
 // One pass: a workgroup takes one row's tile of items, counts the history's entries that fall into it in LDS (whole
 // numbers: any order of the atomics gives the same counts) and streams the tile through registers, in fp32, rounded once.
 // Bound by the table's read and write; the counts cost an LDS word per item, the history a read per tile from the L2.
-// 4096 x 65537 bf16 with 300 entries of history a row: 1.08 GB in 250 us (4.3 TB/s, a copy's rate is 4.7); 1024 x 31232 fp32:
+// 4096 x 65537 bf16 with 300 entries of history a row: 1.08 GB in 250 us (4.3 TB/s, a copy's rate is 4.7; traced: 266); 1024 x 31232 fp32:
 // 256 MB in 44 us; one row of 31232: 4.8 us, a launch and three dependent loads.  Several rows or tiles a workgroup (fewer,
 // longer ones) were measured and no faster.
 #include "dg_internal.h"

@@ -1087,8 +1087,8 @@ def adjust_scores(scores: torch.Tensor, *, history=None, rows: Optional[torch.Te
     presence: a number or float32 [rows].  bias: float32 [items] or [rows, items].  allowed: int32 words of 32 items, bit
     v % 32 of word v // 32 set where item v stays, [words] for all rows or [masks, words] with allowed_rows (int32 [rows]; a
     row whose number is not that of a mask has none; default: mask r for row r).  A row whose mask leaves nothing is all
-    `fill`.  out: where to (scores itself: in place).  Not recorded by autograd, so neither scores, bias and penalties nor
-    out may ask for a gradient where one is recorded."""
+    `fill`.  out: where to (scores itself: in place; otherwise memory that the call reads nothing from).  Not recorded by
+    autograd, so neither scores, bias and penalties nor out may ask for a gradient where one is recorded."""
     n, items, pitch, code = _rows(scores, "scores")
     at, given = scores.get_device(), out is not None
     if not given:

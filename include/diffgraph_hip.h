@@ -723,7 +723,7 @@ int dg_embedding_grad(const void *d_out, int64_t row_stride, const void *ids, in
  * in fp32, rounded once (a fill beyond the type's range becomes an infinity).  What masked places hold does not matter;
  * a row whose mask leaves nothing is all fill.
  *   scores, out       DEVICE, dtype DG_F32 / DG_BF16 / DG_F16, rows row_stride / out_stride elements apart; out may be
- *                     scores (same stride), and must not overlap it otherwise
+ *                     scores (same stride), and must not overlap it otherwise, nor anything else that the call reads
  *   hist_rowptr, hist_col   DEVICE int32 CSR of n_hist rows and n_hist_items entries, any order, repeats counted (NULL:
  *                     no history); ids outside [0, n_items) are passed over.  hist_rows: DEVICE int64[n_rows], the CSR
  *                     row of a score row (NULL: its own number; outside [0, n_hist): no history)
