@@ -113,7 +113,8 @@ def all_rank_topk(usr: torch.Tensor, itm: torch.Tensor, users: torch.Tensor, trn
             scores = ops.adjust_scores(scores, history=history, rows=u, exclude=True, fill=_MASKED, out=None if recorded else scores)
         v, i = torch.topk(scores, min(topk, n_item))
         if recorded:                        # the same values as elements of the product; a masked one is a constant
-            v = torch.where(v == torch.full_like(v, _MASKED), v, preds.gather(1, i))
+            out = torch.full((), _MASKED, device=v.device).to(v.dtype)                # (rounded as the kernel does: -inf in float16)
+            v = torch.where(v == out, v, preds.gather(1, i))
         vals.append(v)
         idx.append(i.to(torch.int32))
     return torch.cat(vals), torch.cat(idx)

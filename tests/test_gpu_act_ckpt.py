@@ -520,7 +520,7 @@ def test_wide_evaluation_takes_interactions_of_either_width(rowptr_type, col_typ
 
 
 @gpu
-@pytest.mark.parametrize("dtype", [torch.float32, torch.float64, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64, torch.bfloat16, torch.float16], ids=str)
 def test_wide_evaluation_passes_gradients_to_its_tables(dtype):
     """The values are scores of the tables, and differentiable in them as torch's mm, mask and topk are: d usr[u] = sum of
     d value * itm[item], nothing through a masked place; with gradients off the same values and items."""
