@@ -132,6 +132,8 @@ extern "C" int dg_adjust_scores(const dg_score_task *t, void *stream) {
   if (!t->scores || !t->out) return dg_fail(DG_ERR_ARG, "dg_adjust_scores: NULL argument");
   if (t->n_rows > 1 && (t->row_stride < 0 || t->out_stride < t->n_items))
     return dg_fail(DG_ERR_ARG, "dg_adjust_scores: rows of the output overlap, or a negative row stride");
+  if (t->n_rows > 1 && t->scores == t->out && t->row_stride != t->out_stride)
+    return dg_fail(DG_ERR_ARG, "dg_adjust_scores: the output overlaps the scores with another row stride");
   if ((t->hist_rowptr != nullptr) != (t->hist_col != nullptr) || (!t->hist_rowptr && t->hist_rows))
     return dg_fail(DG_ERR_ARG, "dg_adjust_scores: a history needs row offsets and item ids");
   if (t->hist_rowptr && (t->n_hist < 0 || t->n_hist_items < 0 || (!t->hist_rows && t->n_hist < t->n_rows)))

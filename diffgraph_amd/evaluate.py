@@ -61,7 +61,7 @@ def all_rank_topk(usrEmbeds: torch.Tensor, itmEmbeds: torch.Tensor, users: torch
     for nm, t in (("usrEmbeds", usrEmbeds), ("itmEmbeds", itmEmbeds)):
         if not t.is_cuda or t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] < 1 or t.shape[1] != usrEmbeds.shape[1]:
             raise DiffGraphHipError(f"{nm}: expected a float32 GPU tensor [rows, latdim], both of one width")
-    if usrEmbeds.shape[1] > DG_D:    # wider than the scoring kernel's rows: torch's mm + topk over mask rows built on the device
+    if usrEmbeds.shape[1] > DG_D:    # wider than the scoring kernel's rows: torch's mm and topk, the training items taken out between them
         from . import wide
         if usrEmbeds.shape[0] != data.n_user or itmEmbeds.shape[0] != data.n_item:
             raise DiffGraphHipError("embedding tables do not match the interaction matrices")

@@ -323,6 +323,13 @@ def test_penalties_and_outputs_that_ask_for_a_gradient(name):
         ops.adjust_scores(s, bias=[0.0] * 64)
 
 
+def test_c_entry_refuses_one_table_with_two_strides():
+    import ctypes as C
+    p = 1 << 20
+    t = _lib.ScoreTask(scores=p, out=p, row_stride=16, out_stride=8, n_rows=2, n_items=8, repetition_all=1.0)
+    assert _lib.load().dg_adjust_scores(C.byref(t), None) == -1 and b"overlap" in _lib.load().dg_last_error()
+
+
 def test_c_entry_names_the_words_of_the_longest_mask():
     import ctypes as C
     items, p = (1 << 31) - 1, 1 << 20
