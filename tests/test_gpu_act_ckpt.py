@@ -592,3 +592,22 @@ def test_recommendations_out_of_trained_tables_are_the_best_that_are_left():
             best = scores[r, left].topk(n).values
             assert bool(((scores[r, i[:n].long()] - v[:n].double()).abs() <= off).all()) and bool(((best - v[:n].double()).abs() <= off).all())
             assert bool((v[1:n] <= v[:n - 1]).all()) if n > 1 else True
+
+
+@gpu
+@pytest.mark.parametrize("use_graph", [False, True])
+@pytest.mark.parametrize("fmt,dims,latdim", [("int8", "[128, 32]", 64), ("e4m3", "[64]", 128)])
+def test_nc_epochs_with_kept_activations(fmt, dims, latdim, use_graph):
+    """The classification model's denoiser with args.act_ckpt, eagerly and with the step recorded."""
+    from diffgraph_amd.train_nc import NCCoach
+    from tests.test_gpu_train import _nc_handler
+    args = copy.copy(dg.nc.DEFAULT_ARGS)
+    args.dims, args.d_emb_size, args.latdim, args.batch, args.act_ckpt = dims, 8, latdim, 8, fmt
+    torch.manual_seed(3)
+    c = NCCoach(_nc_handler(), args, device=DEV, use_graph=use_graph, seed=3)
+    lines = []
+    res = c.run(epochs=2, log=lines.append)
+    dn = c.model.user_denoise_model
+    assert dn.act_ckpt == fmt and not dn.fused
+    assert len(lines) == 2 and all("nan" not in ln.lower() for ln in lines) and 0.0 <= res["macro"] <= 1.0
+    assert all(bool(p.isfinite().all()) for p in c.model.parameters())
