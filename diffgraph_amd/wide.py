@@ -97,7 +97,7 @@ def all_rank_topk(usr: torch.Tensor, itm: torch.Tensor, users: torch.Tensor, trn
     if trn_col.numel() > 0x7fffffff:
         raise DiffGraphHipError(f"trn_col: at most 2^31 - 1 interactions, got {trn_col.numel()}")
     history = (trn_rowptr.to(torch.int32) if trn_rowptr.dtype != torch.int32 else trn_rowptr,
-               trn_col.clamp(-1, n_item).to(torch.int32) if trn_col.dtype != torch.int32 else trn_col)   # (in int32, the kernel's)
+               trn_col.long().clamp(-1, n_item).to(torch.int32) if trn_col.dtype != torch.int32 else trn_col)   # (in int32, the kernel's)
     recorded = torch.is_grad_enabled() and (usr.requires_grad or itm.requires_grad)
     usr = usr if usr.stride(1) == 1 else usr.contiguous()
     vals, idx = [], []

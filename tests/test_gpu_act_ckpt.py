@@ -611,3 +611,17 @@ def test_nc_epochs_with_kept_activations(fmt, dims, latdim, use_graph):
     assert dn.act_ckpt == fmt and not dn.fused
     assert len(lines) == 2 and all("nan" not in ln.lower() for ln in lines) and 0.0 <= res["macro"] <= 1.0
     assert all(bool(p.isfinite().all()) for p in c.model.parameters())
+
+
+@gpu
+@pytest.mark.parametrize("col_type", [torch.uint8, torch.int16])
+def test_wide_evaluation_takes_interactions_in_short_types(col_type):
+    from diffgraph_amd import wide
+    ni = 200 if col_type == torch.uint8 else 40000               # (more items than the type's numbers: none of them interacted with)
+    g = torch.Generator().manual_seed(6)
+    usr, itm = torch.randn(3, 80, generator=g).to(DEV), torch.randn(ni, 80, generator=g).to(DEV)
+    rowptr, col = torch.tensor([0, 2, 2, 5], device=DEV), torch.tensor([0, 7, 100, 3, 120], device=DEV)
+    users = torch.tensor([2, 0, 1], device=DEV)
+    want = wide.all_rank_topk(usr, itm, users, rowptr, col, 9)
+    got = wide.all_rank_topk(usr, itm, users, rowptr.to(torch.int16), col.to(col_type), 9)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
